@@ -229,8 +229,8 @@ def _own(s):
         return s["kcs"], s["vcs"]
     if s["op"] == "beam":
         rows, lens, counts = paged.fork_sequences(s["tables"], s["lens"], s["parents"], s["counts"], s["kcs"], s["vcs"])
-        room, granted, counts = paged.extend_sequences(rows, lens, s["wanted"], counts)
-        counts = paged.free_sequences(s["tables"], s["lens"], s["rows"], counts)
+        room, granted, counts = paged.extend_sequences(rows, lens, s["wanted"], counts, c["block"])
+        counts = paged.free_sequences(s["tables"], s["lens"], s["rows"], counts, c["block"])
         return rows, lens, room, granted, counts, s["kcs"], s["vcs"]
     tables, counts, used = paged.compact_pages(s["tables"], s["lens"], s["counts"], s["kcs"], s["vcs"])
     return tables, counts, used, s["kcs"], s["vcs"]
