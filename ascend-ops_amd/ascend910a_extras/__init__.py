@@ -24,5 +24,7 @@ from . import ascend910a_extras_C  # noqa: E402,F401  (loads libaops.so)
 from . import ops  # noqa: E402,F401
 from . import fused  # noqa: E402,F401
 from . import moe  # noqa: E402,F401
+from . import paged  # noqa: E402,F401
+from . import rotary  # noqa: E402,F401
 
-__all__ = ["ops", "fused", "moe", "ascend910a_extras_C", "LIBRARY_PATH"]
+__all__ = ["ops", "fused", "moe", "paged", "rotary", "ascend910a_extras_C", "LIBRARY_PATH"]

@@ -30,6 +30,8 @@ SOURCES = [
     "swiglu.hip",
     "rope.hip",
     "rope_cache.hip",
+    "rotary.hip",
+    "pages.hip",
     "moe.hip",
     "reshape_and_cache.hip",
     "paged_attention.hip",

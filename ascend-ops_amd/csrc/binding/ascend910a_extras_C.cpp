@@ -466,6 +466,228 @@ py::object rope_reshape_and_cache(const Tensor& q, const Tensor& k, const Tensor
   return py::cast(out_q);
 }
 
+// ---- rotary positions ------------------------------------------------------------------------------
+
+std::tuple<Tensor, Tensor> rotary_tables(int64_t max_position, int64_t rotary_dim, double base, int64_t scaling,
+                                         double factor, double original_max_position, double low, double high,
+                                         double attention_factor, const std::optional<Tensor>& pair_factors,
+                                         bool fp32, at::Device device) {
+  const char* name = "rotary_tables";
+  TORCH_CHECK(max_position >= 0 && rotary_dim >= 2 && rotary_dim % 2 == 0, name,
+              ": max_position must not be negative and rotary_dim must be positive and even, got ", max_position, " and ",
+              rotary_dim);
+  TORCH_CHECK(device.is_cuda(), name, ": the tables are built on the GPU device, got ", device);
+  if (device.index() < 0) device = at::Device(device.type(), c10::hip::current_device());
+  if (pair_factors.has_value()) {
+    TORCH_CHECK(pair_factors->dim() == 1 && pair_factors->size(0) == rotary_dim / 2 && pair_factors->is_contiguous(), name,
+                ": pair_factors must be a contiguous [rotary_dim/2] tensor, got ", pair_factors->sizes());
+    require_device(name, {{"pair_factors", *pair_factors, at::kFloat}});
+    TORCH_CHECK(pair_factors->device() == device, name, ": pair_factors must be on the device of the tables");
+  }
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
+  const at::ScalarType dtype = fp32 ? at::kFloat : at::kHalf;
+  Tensor cos = Tensor(at::detail::empty_cuda({max_position, rotary_dim / 2}, dtype, device, std::nullopt));
+  Tensor sin = fresh_like(cos);
+  Launch l(cos);
+  status(name, aops_rotary_tables(dev_ptr(cos), dev_ptr(sin), fp32, max_position, rotary_dim, base, (int)scaling, factor,
+                                  original_max_position, low, high, attention_factor,
+                                  static_cast<const float*>(dev_ptr(pair_factors)), l.stream));
+  return {cos, sin};
+}
+
+std::tuple<Tensor, Tensor> rotary_embedding(const Tensor& q, const Tensor& k, const Tensor& position_ids,
+                                            const Tensor& cos, const Tensor& sin, bool interleaved) {
+  const char* name = "rotary_embedding";
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && position_ids.dim() == 1 && cos.dim() == 2 && sin.dim() == 2, name,
+              ": input tensors must be 3D, 3D, 1D, 2D, and 2D, got ", q.dim(), "D, ", k.dim(), "D, ", position_ids.dim(),
+              "D, ", cos.dim(), "D, ", sin.dim(), "D");
+  const int64_t tokens = q.size(0), num_heads = q.size(1), head_dim = q.size(2), num_kv_heads = k.size(1);
+  TORCH_CHECK(k.size(0) == tokens && k.size(2) == head_dim, name, ": k must match q in tokens and head_dim");
+  TORCH_CHECK(position_ids.size(0) == tokens, name, ": position_ids must have one entry per token, got ",
+              position_ids.size(0), " and ", tokens);
+  TORCH_CHECK(head_dim > 0 && head_dim % 8 == 0, name, ": head_dim must be a multiple of 8, got ", head_dim);
+  TORCH_CHECK(cos.sizes() == sin.sizes() && cos.size(1) > 0 && 2 * cos.size(1) <= head_dim, name,
+              ": cos and sin must be [max_position, rotary_dim/2] with rotary_dim up to head_dim, got ", cos.sizes(), " and ",
+              sin.sizes());
+  TORCH_CHECK(tokens == 0 || cos.size(0) > 0, name, ": cos and sin must have rows");
+  TORCH_CHECK(position_ids.is_contiguous() && cos.is_contiguous() && sin.is_contiguous(), name,
+              ": position_ids, cos and sin must be contiguous");
+  auto strides_ok = [&](const Tensor& x) {  // a stride that is never taken may be anything
+    return x.stride(2) == 1 && (tokens <= 1 || x.stride(0) % 8 == 0) && (x.size(1) <= 1 || x.stride(1) % 8 == 0);
+  };
+  TORCH_CHECK(q.numel() == 0 || strides_ok(q), name, ": the elements of a head of q must be next to each other and its other "
+              "strides multiples of 8, got ", q.strides());
+  TORCH_CHECK(k.numel() == 0 || strides_ok(k), name, ": the elements of a head of k must be next to each other and its other "
+              "strides multiples of 8, got ", k.strides());
+  const bool fp32 = cos.scalar_type() == at::kFloat;
+  require_device(name, {{"q", q, at::kHalf},
+                        {"k", k, at::kHalf},
+                        {"position_ids", position_ids, at::kInt},
+                        {"cos", cos, fp32 ? at::kFloat : at::kHalf},
+                        {"sin", sin, fp32 ? at::kFloat : at::kHalf}});
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(cos.data_ptr()) & 15) == 0 && (reinterpret_cast<uintptr_t>(sin.data_ptr()) & 15) == 0,
+              name, ": cos and sin must be 16-byte aligned");
+  Tensor out_q = fresh(q, q.sizes(), at::kHalf);
+  Tensor out_k = fresh(k, k.sizes(), at::kHalf);
+  Launch l(q);
+  auto token_stride = [&](const Tensor& x) { return tokens > 1 && x.numel() > 0 ? x.stride(0) : 0; };
+  auto head_stride = [](const Tensor& x) { return x.size(1) > 1 && x.numel() > 0 ? x.stride(1) : 0; };
+  status(name, aops_rotary_f16(dev_ptr(q), dev_ptr(k), static_cast<const int32_t*>(dev_ptr(position_ids)), dev_ptr(cos),
+                               dev_ptr(sin), fp32, dev_ptr(out_q), dev_ptr(out_k), tokens, num_heads, num_kv_heads,
+                               head_dim, 2 * cos.size(1), cos.size(0), interleaved, token_stride(q), head_stride(q),
+                               token_stride(k), head_stride(k), l.stream));
+  return {out_q, out_k};
+}
+
+// ---- pages of the caches ---------------------------------------------------------------------------
+
+// The key and value caches of all layers: one geometry, one device.
+struct PageCaches {
+  std::vector<void*> at;
+  int64_t num_blocks = 0, row_elems = 0, block_size = 0;
+  const Tensor* first = nullptr;
+
+  PageCaches(const char* name, const std::vector<Tensor>& keys, const std::vector<Tensor>& values) {
+    for (const auto* list : {&keys, &values})
+      for (const Tensor& c : *list) {
+        TORCH_CHECK(c.dim() == 4 && c.size(3) == 16 && c.size(1) > 0 && c.size(2) > 0, name,
+                    ": caches must be [num_blocks, row/16, block_size, 16], got ", c.sizes());
+        TORCH_CHECK(c.is_contiguous(), name, ": caches must be contiguous");
+        if (!first) first = &c;
+        TORCH_CHECK(c.sizes() == first->sizes(), name, ": all caches must have the same shape, got ", first->sizes(),
+                    " and ", c.sizes());
+        require_device(name, {{"the first cache", *first, at::kHalf}, {"every cache", c, at::kHalf}});
+        at.push_back(dev_ptr(c));
+      }
+    TORCH_CHECK(first, name, ": there must be at least one cache");
+    TORCH_CHECK(at.size() <= 256, name, ": at most 256 caches, got ", at.size());
+    num_blocks = first->size(0);
+    row_elems = first->size(1) * 16;
+    block_size = first->size(2);
+    TORCH_CHECK(num_blocks > 0, name, ": caches must have pages");
+  }
+};
+
+struct IntArg {
+  const char* name;
+  const Tensor& t;
+  int64_t dim;
+};
+
+void require_ints(const char* name, const Tensor* with, std::initializer_list<IntArg> args) {
+  for (const IntArg& a : args) {
+    TORCH_CHECK(a.t.dim() == a.dim && a.t.is_contiguous(), name, ": ", a.name, " must be a contiguous ", a.dim, "D tensor");
+    require_device(name, {{a.name, a.t, at::kInt}});
+    if (!with) with = &a.t;
+    TORCH_CHECK(a.t.device() == with->device(), name, ": all tensors must be on the same device");
+  }
+}
+
+const int32_t* ints(const Tensor& t) { return static_cast<const int32_t*>(dev_ptr(t)); }
+int32_t* ints_out(const Tensor& t) { return static_cast<int32_t*>(dev_ptr(t)); }
+
+void copy_pages(const std::vector<Tensor>& key_caches, const std::vector<Tensor>& value_caches, const Tensor& src_pages,
+                const Tensor& dst_pages) {
+  const char* name = "copy_pages";
+  const PageCaches c(name, key_caches, value_caches);
+  require_ints(name, c.first, {{"src_pages", src_pages, 1}, {"dst_pages", dst_pages, 1}});
+  TORCH_CHECK(src_pages.size(0) == dst_pages.size(0), name, ": src_pages and dst_pages must have the same length, got ",
+              src_pages.size(0), " and ", dst_pages.size(0));
+  Launch l(*c.first);
+  status(name, aops_copy_pages_f16(c.at.data(), (int64_t)c.at.size(), ints(src_pages), ints(dst_pages), src_pages.size(0),
+                                   c.num_blocks, c.row_elems, c.block_size, l.stream));
+}
+
+void check_pool(const char* name, const Tensor& block_tables, const Tensor& context_lens, const Tensor& ref_counts,
+                const PageCaches& c) {
+  require_ints(name, c.first,
+               {{"block_tables", block_tables, 2}, {"context_lens", context_lens, 1}, {"ref_counts", ref_counts, 1}});
+  TORCH_CHECK(context_lens.size(0) == block_tables.size(0), name, ": context_lens must have one entry per row of block_tables");
+  TORCH_CHECK(ref_counts.size(0) == c.num_blocks, name, ": ref_counts must have one entry per page, got ",
+              ref_counts.size(0), " and ", c.num_blocks);
+}
+
+std::tuple<Tensor, Tensor, Tensor> fork_sequences(const Tensor& block_tables, const Tensor& context_lens,
+                                                  const Tensor& parents, const Tensor& ref_counts,
+                                                  const std::vector<Tensor>& key_caches,
+                                                  const std::vector<Tensor>& value_caches) {
+  const char* name = "fork_sequences";
+  const PageCaches c(name, key_caches, value_caches);
+  check_pool(name, block_tables, context_lens, ref_counts, c);
+  require_ints(name, c.first, {{"parents", parents, 1}});
+  const int64_t children = parents.size(0);
+  Tensor child_tables = fresh(parents, {children, block_tables.size(1)}, at::kInt);
+  Tensor child_lens = fresh(parents, {children}, at::kInt);
+  Tensor new_counts = fresh_like(ref_counts);
+  Launch l(*c.first);
+  const size_t ws_bytes = aops_pages_workspace(children, c.num_blocks);
+  TORCH_CHECK(ws_bytes > 0, name, ": unsupported size");
+  Tensor ws = scratch(parents, ws_bytes);
+  status(name, aops_fork_sequences_f16(ints(block_tables), ints(context_lens), block_tables.size(0), block_tables.size(1),
+                                       ints(parents), children, ints(ref_counts), c.num_blocks, c.at.data(),
+                                       (int64_t)c.at.size(), c.row_elems, c.block_size, ints_out(child_tables),
+                                       ints_out(child_lens), ints_out(new_counts), ws.data_ptr(), ws_bytes, l.stream));
+  return {child_tables, child_lens, new_counts};
+}
+
+std::tuple<Tensor, Tensor, Tensor> extend_sequences(const Tensor& block_tables, const Tensor& context_lens,
+                                                    const Tensor& wanted_lens, const Tensor& ref_counts,
+                                                    int64_t block_size) {
+  const char* name = "extend_sequences";
+  require_ints(name, nullptr, {{"block_tables", block_tables, 2}, {"context_lens", context_lens, 1},
+                               {"wanted_lens", wanted_lens, 1}, {"ref_counts", ref_counts, 1}});
+  TORCH_CHECK(block_size > 0, name, ": block_size must be positive, got ", block_size);
+  TORCH_CHECK(context_lens.size(0) == block_tables.size(0) && wanted_lens.size(0) == block_tables.size(0), name,
+              ": context_lens and wanted_lens must have one entry per row of block_tables");
+  Tensor new_tables = fresh_like(block_tables);
+  Tensor granted = fresh_like(context_lens);
+  Tensor new_counts = fresh_like(ref_counts);
+  Launch l(block_tables);
+  const size_t ws_bytes = aops_pages_workspace(block_tables.size(0), ref_counts.size(0));
+  TORCH_CHECK(ws_bytes > 0, name, ": unsupported size");
+  Tensor ws = scratch(block_tables, ws_bytes);
+  status(name, aops_extend_sequences(ints(block_tables), ints(context_lens), ints(wanted_lens), block_tables.size(0),
+                                     block_tables.size(1), block_size, ints(ref_counts), ref_counts.size(0),
+                                     ints_out(new_tables), ints_out(granted), ints_out(new_counts), ws.data_ptr(), ws_bytes,
+                                     l.stream));
+  return {new_tables, granted, new_counts};
+}
+
+Tensor free_sequences(const Tensor& block_tables, const Tensor& context_lens, const Tensor& rows, const Tensor& ref_counts,
+                      int64_t block_size) {
+  const char* name = "free_sequences";
+  require_ints(name, nullptr, {{"block_tables", block_tables, 2}, {"context_lens", context_lens, 1}, {"rows", rows, 1},
+                               {"ref_counts", ref_counts, 1}});
+  TORCH_CHECK(block_size > 0, name, ": block_size must be positive, got ", block_size);
+  TORCH_CHECK(context_lens.size(0) == block_tables.size(0), name, ": context_lens must have one entry per row of block_tables");
+  Tensor new_counts = fresh_like(ref_counts);
+  Launch l(ref_counts);
+  status(name, aops_free_sequences(ints(block_tables), ints(context_lens), block_tables.size(0), block_tables.size(1),
+                                   block_size, ints(rows), rows.size(0), ints(ref_counts), ref_counts.size(0),
+                                   ints_out(new_counts), l.stream));
+  return new_counts;
+}
+
+std::tuple<Tensor, Tensor, Tensor> compact_pages(const Tensor& block_tables, const Tensor& context_lens,
+                                                 const Tensor& ref_counts, const std::vector<Tensor>& key_caches,
+                                                 const std::vector<Tensor>& value_caches) {
+  const char* name = "compact_pages";
+  const PageCaches c(name, key_caches, value_caches);
+  check_pool(name, block_tables, context_lens, ref_counts, c);
+  Tensor new_tables = fresh_like(block_tables);
+  Tensor new_counts = fresh_like(ref_counts);
+  Tensor used = fresh(ref_counts, {1}, at::kInt);
+  Launch l(*c.first);
+  const size_t ws_bytes = aops_pages_workspace(0, c.num_blocks);
+  TORCH_CHECK(ws_bytes > 0, name, ": unsupported size");
+  Tensor ws = scratch(ref_counts, ws_bytes);
+  status(name, aops_compact_pages_f16(ints(block_tables), ints(context_lens), block_tables.size(0), block_tables.size(1),
+                                      ints(ref_counts), c.num_blocks, c.at.data(), (int64_t)c.at.size(), c.row_elems,
+                                      c.block_size, ints_out(new_tables), ints_out(new_counts), ints_out(used),
+                                      ws.data_ptr(), ws_bytes, l.stream));
+  return {new_tables, new_counts, used};
+}
+
 // Stable sort of the flattened routing by expert: (sorted_idx, inverse_idx, group_list)
 std::tuple<Tensor, Tensor, Tensor> moe_sort(const Tensor& topk_ids, int64_t num_experts) {
   TORCH_CHECK((topk_ids.dim() == 1 || topk_ids.dim() == 2) && topk_ids.is_contiguous(),
@@ -543,6 +765,21 @@ PYBIND11_MODULE(ascend910a_extras_C, m) {
         py::arg("position_ids"), py::arg("cos_cache"), py::arg("sin_cache"), py::arg("key_cache"),
         py::arg("value_cache"), py::arg("slot_indices"), py::arg("return_k") = false,
         py::arg("q_norm_weight") = py::none(), py::arg("k_norm_weight") = py::none(), py::arg("epsilon") = 1e-6);
+  m.def("rotary_tables", &rotary_tables, py::arg("max_position"), py::arg("rotary_dim"), py::arg("base"),
+        py::arg("scaling"), py::arg("factor"), py::arg("original_max_position"), py::arg("low"), py::arg("high"),
+        py::arg("attention_factor"), py::arg("pair_factors"), py::arg("fp32"), py::arg("device"));
+  m.def("rotary_embedding", &rotary_embedding, py::arg("q"), py::arg("k"), py::arg("position_ids"), py::arg("cos"),
+        py::arg("sin"), py::arg("interleaved"));
+  m.def("copy_pages", &copy_pages, py::arg("key_caches"), py::arg("value_caches"), py::arg("src_pages"),
+        py::arg("dst_pages"));
+  m.def("fork_sequences", &fork_sequences, py::arg("block_tables"), py::arg("context_lens"), py::arg("parents"),
+        py::arg("ref_counts"), py::arg("key_caches"), py::arg("value_caches"));
+  m.def("extend_sequences", &extend_sequences, py::arg("block_tables"), py::arg("context_lens"), py::arg("wanted_lens"),
+        py::arg("ref_counts"), py::arg("block_size"));
+  m.def("free_sequences", &free_sequences, py::arg("block_tables"), py::arg("context_lens"), py::arg("rows"),
+        py::arg("ref_counts"), py::arg("block_size"));
+  m.def("compact_pages", &compact_pages, py::arg("block_tables"), py::arg("context_lens"), py::arg("ref_counts"),
+        py::arg("key_caches"), py::arg("value_caches"));
   m.def("moe_sort", &moe_sort, py::arg("topk_ids"), py::arg("num_experts"));
   m.def("moe_gather", &moe_gather, py::arg("x"), py::arg("sorted_idx"), py::arg("group_list"), py::arg("topk"));
   m.def("moe_combine", &moe_combine, py::arg("y"), py::arg("inverse_idx"), py::arg("topk_weights"),

@@ -1,0 +1,506 @@
+// Pages of the paged caches [num_blocks, row_elems/16, block_size, 16]: copied, shared between sequences, given out,
+// taken back and packed, for all layers' caches at once and without a word to the host.
+//
+// The state of a pool is one count per page: how many sequences hold it; a page is free where that is not positive.
+// Pages are given out lowest first in the order of the requests, so every result is determined by its inputs.  All
+// operators read their tables and counts and write new ones; only the caches are written in place, and only in pages
+// that no sequence held before.
+//
+// An allocation is two launches.  `pages_plan` is one workgroup that adds up the requests, lists the lowest free
+// pages, and copies the counts: a scan with one running total, a tile of 8192 counts in registers at a time (ranks
+// inside a wave from ballots).  The second launch has a workgroup per row of the tables and, for forks and packing,
+// workgroups that copy page data, each thread with several 128-bit loads in flight.  Bound: the copies by HBM, the
+// rest by the two launches.
+#include <algorithm>
+
+#include "aops_common.h"
+
+namespace aops {
+
+constexpr int kMaxCaches = 256;
+struct Caches {
+  f16* at[kMaxCaches];
+};
+
+// Copies n 16-byte pieces, which `piece(i)` gives the offset (in halfs) of, between two pages of one cache; called by
+// a workgroup of 256 threads.  Four loads of a thread are in flight before its first store.
+template <typename F>
+__device__ __forceinline__ void copy_pieces(const f16* __restrict__ src, f16* __restrict__ dst, uint32_t begin,
+                                            uint32_t end, F piece) {
+  constexpr uint32_t kDeep = 4;
+  for (uint32_t i = begin + threadIdx.x; i < end; i += 256 * kDeep) {
+    f16x8 v[kDeep];
+#pragma unroll
+    for (uint32_t j = 0; j < kDeep; ++j)
+      if (i + 256 * j < end) v[j] = ld128_stream(src + piece(i + 256 * j));
+#pragma unroll
+    for (uint32_t j = 0; j < kDeep; ++j)
+      if (i + 256 * j < end) st128_stream(dst + piece(i + 256 * j), v[j]);
+  }
+}
+
+constexpr uint32_t kCopyPieces = 1024;  // 16 KiB per workgroup
+
+__global__ __launch_bounds__(256) void copy_pages_kernel(Caches caches, const int32_t* __restrict__ src_pages,
+                                                         const int32_t* __restrict__ dst_pages, uint32_t chunks,
+                                                         int32_t num_blocks, int64_t page_elems) {
+  const uint32_t pair = blockIdx.x / chunks, chunk = blockIdx.x - pair * chunks;
+  const int32_t src = src_pages[pair], dst = dst_pages[pair];
+  if (src < 0 || src >= num_blocks || dst < 0 || dst >= num_blocks || src == dst) return;
+  f16* cache = caches.at[blockIdx.y];
+  const uint32_t begin = chunk * kCopyPieces;
+  const uint32_t end = (uint32_t)min((int64_t)begin + kCopyPieces, page_elems / 8);
+  copy_pieces(cache + src * page_elems, cache + dst * page_elems, begin, end, [](uint32_t i) { return (int64_t)i * 8; });
+}
+
+// ------------------------------------------------------------------------------------------- plans
+// What the planning workgroup leaves for the second launch, in the caller's workspace.
+struct PlanOut {
+  int32_t* head;    // [0]: free pages; packing: [1] = pages that move
+  int32_t* before;  // per request: pages asked for by the requests in front of it
+  int32_t* list;    // the free pages, lowest first, as many as are asked for; packing: the holes
+  int32_t* movers;  // packing: the pages that move, and for every page its place among them
+  int32_t* place;
+};
+
+constexpr int kPlanWaves = 16;
+constexpr int kPlanPer = 8;  // counts per lane and tile
+constexpr int kPlanTile = kPlanWaves * kWave * kPlanPer;
+
+// Exclusive sum over the waves of a workgroup and the total; `sums`: kPlanWaves ints of LDS.
+__device__ __forceinline__ int plan_waves_before(int mine, int* sums, int& total) {
+  const int wave = threadIdx.x / kWave;
+  __syncthreads();  // the last round's values have been read
+  if ((threadIdx.x & (kWave - 1)) == 0) sums[wave] = mine;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    const int n = sums[w];
+    before += w < wave ? n : 0;
+    total += n;
+  }
+  return before;
+}
+
+// One pass over the counts in page order: visit(page, count, is_free, free pages in front of it).  Returns the free pages.
+template <typename F>
+__device__ __forceinline__ int plan_scan(const int32_t* __restrict__ counts, int num_blocks, int* sums, F visit) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  const uint64_t below = lane == 0 ? 0 : ~uint64_t(0) >> (kWave - lane);
+  int running = 0;
+  for (int64_t tile = 0; tile < num_blocks; tile += kPlanTile) {
+    const int64_t first = tile + wave * (kWave * kPlanPer) + lane;
+    int32_t c[kPlanPer];
+    uint64_t free[kPlanPer];
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < kPlanPer; ++j) c[j] = first + j * kWave < num_blocks ? counts[first + j * kWave] : 1;
+#pragma unroll
+    for (int j = 0; j < kPlanPer; ++j) {
+      free[j] = __builtin_amdgcn_ballot_w64(c[j] <= 0);
+      mine += __builtin_popcountll(free[j]);
+    }
+    int total;
+    int rank = running + plan_waves_before(mine, sums, total);
+#pragma unroll
+    for (int j = 0; j < kPlanPer; ++j) {
+      if (first + j * kWave < num_blocks)
+        visit((int)(first + j * kWave), c[j], c[j] <= 0, rank + __builtin_popcountll(free[j] & below));
+      rank += __builtin_popcountll(free[j]);
+    }
+    running += total;
+  }
+  return running;
+}
+
+struct Tables {
+  const int32_t* tables;
+  const int32_t* lens;
+  int32_t seqs, width, block_size;
+};
+
+// Tokens of a sequence as far as its row of the table can hold them; 0 for a row that is none.
+__device__ __forceinline__ int seq_tokens(const Tables& t, int seq) {
+  if (seq < 0 || seq >= t.seqs) return 0;
+  return (int)min((int64_t)max(t.lens[seq], 0), (int64_t)t.width * t.block_size);
+}
+__device__ __forceinline__ int pages_of(int64_t tokens, int block_size) {
+  return (int)((tokens + block_size - 1) / block_size);
+}
+
+// Requests: fork asks for one page where the parent's last page is not full, extend for the pages that are missing.
+// `who`: parents, or the wanted lengths.
+template <bool FORK>
+__device__ __forceinline__ int plan_request(const Tables& t, const int32_t* who, int i) {
+  if constexpr (FORK) {
+    return seq_tokens(t, who[i]) % t.block_size != 0;
+  } else {
+    const int have = seq_tokens(t, i), want = who[i];
+    if (want <= have || (int64_t)want > (int64_t)t.width * t.block_size) return 0;
+    return pages_of(want, t.block_size) - pages_of(have, t.block_size);
+  }
+}
+
+template <bool FORK>
+__global__ __launch_bounds__(kPlanWaves* kWave) void pages_plan_kernel(Tables t, const int32_t* __restrict__ who,
+                                                                       int32_t requests,
+                                                                       const int32_t* __restrict__ counts,
+                                                                       int32_t num_blocks, int32_t* __restrict__ new_counts,
+                                                                       PlanOut out) {
+  __shared__ int sums[kPlanWaves];
+  const int lane = threadIdx.x & (kWave - 1);
+  // Sums of requests stop at num_blocks + 1: what is beyond is refused all the same, and nothing overflows.
+  const int cap = num_blocks == 0x7fffffff ? num_blocks : num_blocks + 1;
+  int asked = 0;
+  for (int64_t tile = 0; tile < requests; tile += kPlanWaves * kWave) {
+    const int64_t i = tile + threadIdx.x;
+    const int need = i < requests ? plan_request<FORK>(t, who, (int)i) : 0;
+    int64_t upto = need;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int64_t o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
+    }
+    const int wave_total = (int)min(__shfl(upto, kWave - 1), (int64_t)cap);
+    int64_t before = 0, total = 0;
+    {
+      const int wave = threadIdx.x / kWave;
+      __syncthreads();
+      if (lane == 0) sums[wave] = wave_total;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kPlanWaves; ++w) {
+        before += w < wave ? sums[w] : 0;
+        total += sums[w];
+      }
+    }
+    if (i < requests) out.before[i] = (int)min((int64_t)asked + before + (upto - need), (int64_t)cap);
+    asked = (int)min((int64_t)asked + total, (int64_t)cap);
+  }
+  const int free = plan_scan(counts, num_blocks, sums, [&](int page, int32_t c, bool is_free, int rank) {
+    new_counts[page] = max(c, 0);
+    if (is_free && rank < asked) out.list[rank] = page;
+  });
+  if (threadIdx.x == 0) out.head[0] = free;
+}
+
+// ------------------------------------------------------------------------------------------- fork
+// Workgroup (child, y): y == 0 writes the child's row; y - 1 = cache * slices + slice copies a slice of the used tokens
+// of the parent's last page.
+__global__ __launch_bounds__(256) void fork_kernel(Tables t, const int32_t* __restrict__ parents, Caches caches,
+                                                   uint32_t slices, int32_t num_blocks, uint32_t granules,
+                                                   int32_t* __restrict__ child_tables, int32_t* __restrict__ child_lens,
+                                                   int32_t* __restrict__ new_counts, PlanOut plan) {
+  const int child = blockIdx.x;
+  const int parent = parents[child];
+  const int tokens = seq_tokens(t, parent);
+  const int full = tokens / t.block_size, part = tokens - full * t.block_size;
+  const int rank = plan.before[child];
+  const bool ok = part == 0 || rank < plan.head[0];
+  const int32_t* row = t.tables + (int64_t)(tokens > 0 ? parent : 0) * t.width;
+  if (blockIdx.y == 0) {
+    int32_t* out = child_tables + (int64_t)child * t.width;
+    for (int j = threadIdx.x; j < t.width; j += 256) {
+      int32_t page = -1;
+      if (ok && j < full) page = row[j];
+      if (ok && j == full && part > 0) page = plan.list[rank];
+      out[j] = page;
+      if (ok && j < full + (part > 0) && page >= 0 && page < num_blocks) atomicAdd(new_counts + page, 1);
+    }
+    if (threadIdx.x == 0) child_lens[child] = ok ? tokens : 0;
+    return;
+  }
+  if (!ok || part == 0) return;
+  const int32_t src = row[full];
+  if (src < 0 || src >= num_blocks) return;
+  const int64_t page_elems = (int64_t)granules * t.block_size * 16;
+  const int64_t from = src * page_elems, to = plan.list[rank] * page_elems;
+  const uint32_t per_granule = 2u * part;  // 16-byte pieces of the used tokens; a page has `granules` such runs
+  const uint32_t pieces = granules * per_granule;
+  const uint32_t cache = (blockIdx.y - 1) / slices, slice = (blockIdx.y - 1) - cache * slices;
+  f16* base = caches.at[cache];
+  const uint32_t begin = (uint32_t)((uint64_t)pieces * slice / slices);
+  const uint32_t end = (uint32_t)((uint64_t)pieces * (slice + 1) / slices);
+  copy_pieces(base + from, base + to, begin, end, [&](uint32_t i) {
+    const uint32_t c = i / per_granule;
+    return ((int64_t)c * t.block_size * 2 + (i - c * per_granule)) * 8;
+  });
+}
+
+// ------------------------------------------------------------------------------------------- extend
+__global__ __launch_bounds__(256) void extend_kernel(Tables t, const int32_t* __restrict__ wanted,
+                                                     int32_t* __restrict__ new_tables, int32_t* __restrict__ granted,
+                                                     int32_t* __restrict__ new_counts, PlanOut plan) {
+  const int seq = blockIdx.x;
+  const int have_tokens = seq_tokens(t, seq), want = wanted[seq];
+  const int have = pages_of(have_tokens, t.block_size);
+  const int need = plan_request<false>(t, wanted, seq);
+  const int before = plan.before[seq];
+  const bool ok = want > have_tokens && (int64_t)want <= (int64_t)t.width * t.block_size &&
+                  (need == 0 || (int64_t)before + need <= plan.head[0]);
+  const int32_t* row = t.tables + (int64_t)seq * t.width;
+  int32_t* out = new_tables + (int64_t)seq * t.width;
+  for (int j = threadIdx.x; j < t.width; j += 256) {
+    int32_t page = row[j];
+    if (ok && j >= have && j < have + need) {
+      page = plan.list[before + j - have];
+      atomicAdd(new_counts + page, 1);
+    }
+    out[j] = page;
+  }
+  if (threadIdx.x == 0) granted[seq] = ok ? want : have_tokens;
+}
+
+// ------------------------------------------------------------------------------------------- free
+__global__ __launch_bounds__(256) void counts_copy_kernel(const int32_t* __restrict__ counts, int32_t num_blocks,
+                                                          int32_t* __restrict__ new_counts) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < num_blocks) new_counts[i] = max(counts[i], 0);
+}
+
+// A count never falls below zero: a decrement that finds none left is taken back.  As many succeed as there were
+// counts, in whatever order they come: one fails only after all have been taken.
+__global__ __launch_bounds__(256) void free_kernel(Tables t, const int32_t* __restrict__ rows, int32_t num_blocks,
+                                                   int32_t* __restrict__ new_counts) {
+  const int seq = rows[blockIdx.x];
+  const int pages = pages_of(seq_tokens(t, seq), t.block_size);
+  const int32_t* row = t.tables + (int64_t)(pages > 0 ? seq : 0) * t.width;
+  for (int j = threadIdx.x; j < pages; j += 256) {
+    const int32_t page = row[j];
+    if (page < 0 || page >= num_blocks) continue;
+    if (atomicSub(new_counts + page, 1) <= 0) atomicAdd(new_counts + page, 1);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- compact
+__global__ __launch_bounds__(kPlanWaves* kWave) void compact_plan_kernel(const int32_t* __restrict__ counts,
+                                                                         int32_t num_blocks, int32_t* __restrict__ used_out,
+                                                                         PlanOut out) {
+  __shared__ int sums[kPlanWaves];
+  const int free = plan_scan(counts, num_blocks, sums, [](int, int32_t, bool, int) {});
+  const int used = num_blocks - free;
+  __shared__ int free_below;  // free pages in front of page `used`: the holes
+  if (threadIdx.x == 0) free_below = used == num_blocks ? free : -1;
+  plan_scan(counts, num_blocks, sums, [&](int page, int32_t, bool is_free, int rank) {
+    if (page == used) free_below = rank;
+    if (is_free && page < used) out.list[rank] = page;
+    // used pages in front of this one: page - rank; the ones behind `used` come after used - free_below others
+    if (!is_free && page >= used) out.place[page] = page - rank;
+  });
+  __syncthreads();
+  const int holes = free_below, stay = used - holes;
+  for (int64_t p = (int64_t)used + threadIdx.x; p < num_blocks; p += kPlanWaves * kWave) {
+    if (counts[p] <= 0) continue;
+    const int k = out.place[p] - stay;
+    out.place[p] = k;
+    out.movers[k] = (int)p;
+  }
+  if (threadIdx.x == 0) {
+    out.head[0] = used;
+    out.head[1] = holes;
+    used_out[0] = used;
+  }
+}
+
+// Workgroups 0 .. row_wgs-1 rewrite the tables and counts, the others copy pages.
+__global__ __launch_bounds__(256) void compact_kernel(Tables t, const int32_t* __restrict__ counts, int32_t num_blocks,
+                                                      Caches caches, int32_t num_caches, uint32_t chunks,
+                                                      int64_t page_elems, uint32_t row_wgs, int32_t* __restrict__ new_tables,
+                                                      int32_t* __restrict__ new_counts, PlanOut plan) {
+  const int used = plan.head[0], moves = plan.head[1];
+  if (blockIdx.x < row_wgs) {
+    const int64_t stride = (int64_t)row_wgs * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t entries = (int64_t)t.seqs * t.width;
+    for (int64_t i = first; i < entries; i += stride) {
+      const int seq = (int)(i / t.width), j = (int)(i - (int64_t)seq * t.width);
+      int32_t page = t.tables[i];
+      if (page >= used && page < num_blocks && j < pages_of(seq_tokens(t, seq), t.block_size) && counts[page] > 0)
+        page = plan.list[plan.place[page]];
+      new_tables[i] = page;
+    }
+    for (int64_t p = first; p < num_blocks; p += stride) {
+      const int32_t c = counts[p];
+      if (p >= used) {
+        new_counts[p] = 0;
+        if (c > 0) new_counts[plan.list[plan.place[p]]] = c;
+      } else if (c > 0) {
+        new_counts[p] = c;
+      }
+    }
+    return;
+  }
+  const uint64_t per_move = (uint64_t)num_caches * chunks;
+  const uint64_t items = per_move * moves;
+  for (uint64_t i = blockIdx.x - row_wgs; i < items; i += gridDim.x - row_wgs) {
+    const uint32_t move = (uint32_t)(i / per_move), rest = (uint32_t)(i - move * per_move);
+    const uint32_t cache = rest / chunks, chunk = rest - cache * chunks;
+    const uint32_t begin = chunk * kCopyPieces;
+    const uint32_t end = (uint32_t)min((int64_t)begin + kCopyPieces, page_elems / 8);
+    f16* base = caches.at[cache];
+    copy_pieces(base + plan.movers[move] * page_elems, base + plan.list[move] * page_elems, begin, end,
+                [](uint32_t j) { return (int64_t)j * 8; });
+  }
+}
+
+// ------------------------------------------------------------------------------------------- host side
+static int fill(Caches& c, void* const* caches, int64_t num_caches) {
+  if (!caches) return AOPS_ERR_INVALID_ARGUMENT;
+  for (int64_t i = 0; i < num_caches; ++i) {
+    if (!caches[i]) return AOPS_ERR_INVALID_ARGUMENT;
+    c.at[i] = static_cast<f16*>(caches[i]);
+  }
+  return AOPS_OK;
+}
+
+static bool geometry_ok(int64_t num_caches, int64_t num_blocks, int64_t row_elems, int64_t block_size) {
+  return num_caches >= 1 && num_caches <= kMaxCaches && num_blocks >= 0 && num_blocks < 0x7fffffff && row_elems > 0 &&
+         row_elems % 16 == 0 && row_elems <= 0x7fffffff && block_size > 0 && block_size <= 0x7fffffff &&
+         row_elems * block_size / 8 <= 0x7fffffff;  // 16-byte pieces of a page are counted in 32 bits
+}
+
+static bool tables_ok(int64_t seqs, int64_t max_pages, int64_t block_size) {
+  return seqs >= 0 && seqs <= 0x7fffffff && max_pages >= 0 && max_pages <= 0x7fffffff && block_size > 0 &&
+         block_size <= 0x7fffffff;
+}
+
+static PlanOut plan_layout(void* workspace, int64_t num_blocks) {
+  int32_t* w = static_cast<int32_t*>(workspace);
+  PlanOut p;
+  p.head = w;
+  p.list = w + 4;
+  p.before = p.list + num_blocks;
+  p.movers = p.before;  // packing has no requests
+  p.place = p.movers + num_blocks;
+  return p;
+}
+
+static uint32_t page_chunks(int64_t page_elems) { return (uint32_t)((page_elems / 8 + kCopyPieces - 1) / kCopyPieces); }
+
+}  // namespace aops
+
+extern "C" size_t aops_pages_workspace(int64_t requests, int64_t num_blocks) {
+  if (requests < 0 || num_blocks < 0 || requests > 0x7fffffff || num_blocks >= 0x7fffffff) return 0;
+  const int64_t ints = 4 + num_blocks + std::max(requests, 2 * num_blocks);
+  return (size_t)ints * sizeof(int32_t);
+}
+
+extern "C" int aops_copy_pages_f16(void* const* caches, int64_t num_caches, const int32_t* src_pages,
+                                   const int32_t* dst_pages, int64_t pairs, int64_t num_blocks, int64_t row_elems,
+                                   int64_t block_size, void* stream) {
+  using namespace aops;
+  if (!geometry_ok(num_caches, num_blocks, row_elems, block_size) || pairs < 0) return AOPS_ERR_INVALID_ARGUMENT;
+  if (pairs == 0 || num_blocks == 0) return AOPS_OK;
+  const uint32_t chunks = page_chunks(row_elems * block_size);
+  if (pairs > 0x7fffffff / (int64_t)chunks || !src_pages || !dst_pages) return AOPS_ERR_INVALID_ARGUMENT;
+  Caches c;
+  if (const int e = fill(c, caches, num_caches)) return e;
+  copy_pages_kernel<<<dim3((unsigned)(pairs * chunks), (unsigned)num_caches), 256, 0, static_cast<hipStream_t>(stream)>>>(
+      c, src_pages, dst_pages, chunks, (int32_t)num_blocks, row_elems * block_size);
+  return record_launch_status(hipGetLastError());
+}
+
+extern "C" int aops_fork_sequences_f16(const int32_t* block_tables, const int32_t* context_lens, int64_t seqs,
+                                       int64_t max_pages, const int32_t* parents, int64_t children,
+                                       const int32_t* ref_counts, int64_t num_blocks, void* const* caches,
+                                       int64_t num_caches, int64_t row_elems, int64_t block_size, int32_t* child_tables,
+                                       int32_t* child_lens, int32_t* new_ref_counts, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  using namespace aops;
+  if (!geometry_ok(num_caches, num_blocks, row_elems, block_size) || !tables_ok(seqs, max_pages, block_size) ||
+      children < 0 || children > 0x7fffffff)
+    return AOPS_ERR_INVALID_ARGUMENT;
+  if (children == 0 && num_blocks == 0) return AOPS_OK;
+  if ((num_blocks > 0 && (!ref_counts || !new_ref_counts)) ||
+      (children > 0 && (!parents || !child_lens || (max_pages > 0 && !child_tables))) ||
+      (seqs > 0 && (!context_lens || (max_pages > 0 && !block_tables))))
+    return AOPS_ERR_INVALID_ARGUMENT;
+  Caches c;
+  if (const int e = fill(c, caches, num_caches)) return e;
+  if (!workspace || workspace_bytes < aops_pages_workspace(children, num_blocks)) return AOPS_ERR_WORKSPACE;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
+  const PlanOut plan = plan_layout(workspace, num_blocks);
+  pages_plan_kernel<true><<<1, kPlanWaves * kWave, 0, st>>>(t, parents, (int32_t)children, ref_counts,
+                                                            (int32_t)num_blocks, new_ref_counts, plan);
+  // a slice is at most four rounds of a workgroup's copy loop, unless a page is larger than 64 of them
+  const uint32_t slices = (uint32_t)std::min<int64_t>((row_elems * block_size / 8 + 4 * kCopyPieces - 1) / (4 * kCopyPieces), 64);
+  if (children > 0)
+    fork_kernel<<<dim3((unsigned)children, 1 + (unsigned)num_caches * slices), 256, 0, st>>>(
+        t, parents, c, slices, (int32_t)num_blocks, (uint32_t)(row_elems / 16), child_tables, child_lens, new_ref_counts,
+        plan);
+  return record_launch_status(hipGetLastError());
+}
+
+extern "C" int aops_extend_sequences(const int32_t* block_tables, const int32_t* context_lens,
+                                     const int32_t* wanted_lens, int64_t seqs, int64_t max_pages, int64_t block_size,
+                                     const int32_t* ref_counts, int64_t num_blocks, int32_t* new_tables,
+                                     int32_t* granted_lens, int32_t* new_ref_counts, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  using namespace aops;
+  if (!tables_ok(seqs, max_pages, block_size) || num_blocks < 0 || num_blocks >= 0x7fffffff)
+    return AOPS_ERR_INVALID_ARGUMENT;
+  if (seqs == 0 && num_blocks == 0) return AOPS_OK;
+  if ((num_blocks > 0 && (!ref_counts || !new_ref_counts)) ||
+      (seqs > 0 && (!context_lens || !wanted_lens || !granted_lens || (max_pages > 0 && (!block_tables || !new_tables)))))
+    return AOPS_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < aops_pages_workspace(seqs, num_blocks)) return AOPS_ERR_WORKSPACE;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
+  const PlanOut plan = plan_layout(workspace, num_blocks);
+  pages_plan_kernel<false><<<1, kPlanWaves * kWave, 0, st>>>(t, wanted_lens, (int32_t)seqs, ref_counts,
+                                                             (int32_t)num_blocks, new_ref_counts, plan);
+  if (seqs > 0)
+    extend_kernel<<<(unsigned)seqs, 256, 0, st>>>(t, wanted_lens, new_tables, granted_lens, new_ref_counts, plan);
+  return record_launch_status(hipGetLastError());
+}
+
+extern "C" int aops_free_sequences(const int32_t* block_tables, const int32_t* context_lens, int64_t seqs,
+                                   int64_t max_pages, int64_t block_size, const int32_t* rows, int64_t num_rows,
+                                   const int32_t* ref_counts, int64_t num_blocks, int32_t* new_ref_counts, void* stream) {
+  using namespace aops;
+  if (!tables_ok(seqs, max_pages, block_size) || num_rows < 0 || num_rows > 0x7fffffff || num_blocks < 0 ||
+      num_blocks >= 0x7fffffff)
+    return AOPS_ERR_INVALID_ARGUMENT;
+  if (num_blocks == 0) return AOPS_OK;
+  if (!ref_counts || !new_ref_counts || (num_rows > 0 && !rows) ||
+      (seqs > 0 && (!context_lens || (max_pages > 0 && !block_tables))))
+    return AOPS_ERR_INVALID_ARGUMENT;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
+  counts_copy_kernel<<<(unsigned)((num_blocks + 255) / 256), 256, 0, st>>>(ref_counts, (int32_t)num_blocks, new_ref_counts);
+  if (num_rows > 0 && seqs > 0 && max_pages > 0)
+    free_kernel<<<(unsigned)num_rows, 256, 0, st>>>(t, rows, (int32_t)num_blocks, new_ref_counts);
+  return record_launch_status(hipGetLastError());
+}
+
+extern "C" int aops_compact_pages_f16(const int32_t* block_tables, const int32_t* context_lens, int64_t seqs,
+                                      int64_t max_pages, const int32_t* ref_counts, int64_t num_blocks,
+                                      void* const* caches, int64_t num_caches, int64_t row_elems, int64_t block_size,
+                                      int32_t* new_tables, int32_t* new_ref_counts, int32_t* num_used, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  using namespace aops;
+  if (!geometry_ok(num_caches, num_blocks, row_elems, block_size) || !tables_ok(seqs, max_pages, block_size))
+    return AOPS_ERR_INVALID_ARGUMENT;
+  if (!num_used || (num_blocks > 0 && (!ref_counts || !new_ref_counts)) ||
+      (seqs > 0 && (!context_lens || (max_pages > 0 && (!block_tables || !new_tables)))))
+    return AOPS_ERR_INVALID_ARGUMENT;
+  Caches c;
+  if (const int e = fill(c, caches, num_caches)) return e;
+  if (!workspace || workspace_bytes < aops_pages_workspace(0, num_blocks)) return AOPS_ERR_WORKSPACE;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
+  const PlanOut plan = plan_layout(workspace, num_blocks);
+  compact_plan_kernel<<<1, kPlanWaves * kWave, 0, st>>>(ref_counts, (int32_t)num_blocks, num_used, plan);
+  const int64_t page_elems = row_elems * block_size;
+  const uint32_t chunks = page_chunks(page_elems);
+  const int64_t ints = std::max(seqs * max_pages, num_blocks);
+  const int64_t row_wgs = std::min<int64_t>(std::max<int64_t>((ints + 1023) / 1024, 1), device_cu_count());
+  const int64_t most = num_blocks / 2 * num_caches * (int64_t)chunks;  // at most half of the pages move
+  const int64_t copy_wgs = std::min<int64_t>(most, 8 * (int64_t)device_cu_count());
+  compact_kernel<<<(unsigned)(row_wgs + std::max<int64_t>(copy_wgs, 1)), 256, 0, st>>>(
+      t, ref_counts, (int32_t)num_blocks, c, (int32_t)num_caches, chunks, page_elems, (uint32_t)row_wgs, new_tables,
+      new_ref_counts, plan);
+  return record_launch_status(hipGetLastError());
+}

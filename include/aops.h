@@ -126,6 +126,107 @@ int aops_qknorm_rope_reshape_and_cache_f16(
     int64_t head_dim, int64_t num_blocks, int64_t block_size, void* stream);
 
 /*
+ * cos and sin tables [max_position, rotary_dim/2] (fp16, or fp32 with table_fp32) of the angles p * f_j,
+ * f_j = base^(-2j/rotary_dim), formed in 64 bits; every entry times attention_factor.  rotary_dim is even.
+ * scaling changes the frequencies for contexts longer than the model was trained on:
+ *   0  nothing
+ *   1  linear: f_j / factor
+ *   2  a larger base: base * factor^(R/(R-2)), R = rotary_dim > 2
+ *   3  the same with factor * max_position / original_max_position - (factor - 1) in the place of factor where
+ *      max_position > original_max_position, and nothing changed where not
+ *   4  by parts (YaRN, arXiv:2309.00071): pairs that turn more than `low` times (beta_fast, 32) within
+ *      original_max_position keep f_j, pairs that turn less than `high` times (beta_slow, 1) get f_j / factor, in
+ *      between (in pair numbers, rounded outwards) a linear mix
+ *   5  by wave length (as Llama 3.1's configuration defines it): f_j / factor below `low` turns within
+ *      original_max_position, f_j above `high` turns, a linear mix in turns in between
+ *   6  f_j / pair_factors[j], pair_factors fp32 [rotary_dim/2] on the device
+ * attention_factor 0 = the scaling's own: 0.1 ln(factor) + 1 for 4, sqrt(1 + ln(factor) / ln(original_max_position))
+ * for 6 (both with factor > 1), 1 otherwise.
+ * No counterpart in the reference, whose callers build one plain table (reference benchmark/test_graph.py:299-317).
+ */
+int aops_rotary_tables(void* cos_out, void* sin_out, int table_fp32, int64_t max_position, int64_t rotary_dim,
+                       double base, int scaling, double factor, double original_max_position, double low, double high,
+                       double attention_factor, const float* pair_factors, void* stream);
+
+/*
+ * Rotary embedding of the first rotary_dim (even) elements of every head of q and k; the others are copied.
+ * interleaved 0: element j is paired with j + rotary_dim/2; 1: 2j with 2j + 1.
+ * q: [tokens, num_heads, head_dim] with the given strides (in elements, multiples of 8, e.g. into a fused projection),
+ * the elements of a head next to each other; k likewise; out_q, out_k: densely packed, not overlapping the inputs.
+ * cos_table, sin_table: [max_position, rotary_dim/2], fp16 or (table_fp32) fp32; position_ids: int32 [tokens], positions
+ * outside the table read its nearest row.  head_dim must be a multiple of 8.
+ * The reference has the case interleaved 0, rotary_dim == head_dim, dense (reference csrc/ffi/ops.cpp:76-83).
+ */
+int aops_rotary_f16(const void* q, const void* k, const int32_t* position_ids, const void* cos_table,
+                    const void* sin_table, int table_fp32, void* out_q, void* out_k, int64_t tokens, int64_t num_heads,
+                    int64_t num_kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t max_position, int interleaved,
+                    int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                    void* stream);
+
+/*
+ * Pages of the paged caches.  `caches`: HOST array of num_caches (1 to 256) device pointers, the key and value caches
+ * of all layers, each [num_blocks, row_elems/16, block_size, 16]; it is read during the call only.  ref_counts: int32
+ * [num_blocks] on the device, the number of sequences that hold a page; a page is free where it is not positive.
+ * block_tables: int32 [seqs, max_pages], context_lens: int32 [seqs]; a sequence holds the first
+ * ceil(context_len / block_size) entries of its row (lengths are limited to 0 .. max_pages * block_size).  Tables and
+ * counts are read, new ones are written to other memory; negative counts come out as 0.  Table entries and page
+ * numbers outside the caches are passed on, and neither counted nor copied.  Pages are given out lowest first, in the
+ * order of the requests.  workspace: aops_pages_workspace(requests, num_blocks) bytes, where requests = children of a
+ * fork, sequences of an extension, 0 for packing.
+ * No counterpart in the reference, which leaves block tables to its caller.
+ */
+size_t aops_pages_workspace(int64_t requests, int64_t num_blocks);
+
+/*
+ * Copies page src_pages[i] to dst_pages[i] (int32, on the device) in every cache.  Pairs that name a page outside the
+ * caches are skipped.  A page that is the destination of two pairs, or source of one and destination of another, ends
+ * up with unspecified contents.
+ */
+int aops_copy_pages_f16(void* const* caches, int64_t num_caches, const int32_t* src_pages, const int32_t* dst_pages,
+                        int64_t pairs, int64_t num_blocks, int64_t row_elems, int64_t block_size, void* stream);
+
+/*
+ * children sequences that begin as copies of parents[i]: a child shares its parent's full pages (their counts go up)
+ * and gets a page of its own for the tokens behind them, into which those tokens are copied in every cache; the rest of
+ * that page is left as it was.  child_tables: int32 [children, max_pages], entries behind the child's pages are -1;
+ * child_lens: int32 [children].  A child for which no free page is left, or whose parent is none of the sequences,
+ * gets length 0, a row of -1 and no pages.
+ */
+int aops_fork_sequences_f16(const int32_t* block_tables, const int32_t* context_lens, int64_t seqs, int64_t max_pages,
+                            const int32_t* parents, int64_t children, const int32_t* ref_counts, int64_t num_blocks,
+                            void* const* caches, int64_t num_caches, int64_t row_elems, int64_t block_size,
+                            int32_t* child_tables, int32_t* child_lens, int32_t* new_ref_counts, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/*
+ * Room for wanted_lens[b] tokens in every sequence: missing pages are given out and entered into new_tables (the other
+ * entries are copied).  granted_lens[b] = wanted_lens[b], or the present length where that is not smaller, where the
+ * row of the table is too short, or where the free pages do not suffice for this and all requests in front of it.
+ */
+int aops_extend_sequences(const int32_t* block_tables, const int32_t* context_lens, const int32_t* wanted_lens,
+                          int64_t seqs, int64_t max_pages, int64_t block_size, const int32_t* ref_counts,
+                          int64_t num_blocks, int32_t* new_tables, int32_t* granted_lens, int32_t* new_ref_counts,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Takes back the pages of the sequences rows[i] (int32 [num_rows]; rows outside the table are skipped): the count of
+ * each goes down by one for every time it is named, never below 0.
+ */
+int aops_free_sequences(const int32_t* block_tables, const int32_t* context_lens, int64_t seqs, int64_t max_pages,
+                        int64_t block_size, const int32_t* rows, int64_t num_rows, const int32_t* ref_counts,
+                        int64_t num_blocks, int32_t* new_ref_counts, void* stream);
+
+/*
+ * Packs the used pages into the lowest page numbers: with `used` of them, the used pages from number `used` on move, in
+ * ascending order, to the free pages below, in ascending order; the tables' live entries and the counts follow.
+ * num_used: int32 [1] on the device.  Pages behind it keep their contents.
+ */
+int aops_compact_pages_f16(const int32_t* block_tables, const int32_t* context_lens, int64_t seqs, int64_t max_pages,
+                           const int32_t* ref_counts, int64_t num_blocks, void* const* caches, int64_t num_caches,
+                           int64_t row_elems, int64_t block_size, int32_t* new_tables, int32_t* new_ref_counts,
+                           int32_t* num_used, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Grouped (per-expert) matmul over expert-sorted rows.
  * x: [rows, k]; w: [num_experts, n, k] (each expert's weight stored N-major, K contiguous --
  * the logical [E, K, N] tensor with stride(1)==1, stride(2)==K); group_list: int64

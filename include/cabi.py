@@ -15,6 +15,7 @@ _SCALARS = {
     "int64_t": ctypes.c_int64,
     "size_t": ctypes.c_size_t,
     "float": ctypes.c_float,
+    "double": ctypes.c_double,
 }
 
 

@@ -1,0 +1,214 @@
+"""Pages of the paged caches, copied, forked, given out, freed and packed on the device, against the same steps on Python
+lists.  Everything is exact."""
+import random
+
+import pytest
+import torch
+
+import oracle.serving_ref as S
+
+pytestmark = pytest.mark.gpu
+H, I = torch.float16, torch.int32
+
+
+@pytest.fixture(scope="module")
+def paged():
+    from ascend910a_extras import paged as p
+
+    return p
+
+
+def _caches(dev, blocks, row, block, layers, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    # bit patterns of every kind, NaN among them: pages are moved, not computed with
+    return [torch.randint(-32768, 32768, (blocks, row // 16, block, 16), generator=g, dtype=torch.int16).view(H).to(dev)
+            for _ in range(2 * layers)]
+
+
+def _same_bits(a, b):
+    return torch.equal(a.cpu().view(torch.int16), b.cpu().view(torch.int16))
+
+
+def _pool(seed, blocks, block, seqs, width, share=0.3, odd=True):
+    """Tables, lengths and counts of a pool in use: shared pages, rows of length zero, lengths beyond the row, entries and
+    counts that are out of range."""
+    r = random.Random(seed)
+    tables = [[r.randrange(-2, blocks + 2) if odd else -1 for _ in range(width)] for _ in range(seqs)]
+    order = list(range(blocks))
+    r.shuffle(order)
+    counts = [0] * blocks
+    lens = []
+    for b in range(seqs):
+        n = r.choice([0, 1, block, block + 1, r.randrange(0, width * block + 1), r.randrange(0, width * block + 1)])
+        for j in range(-(-n // block)):
+            if b and r.random() < share:
+                page = tables[r.randrange(b)][j]
+            elif order:
+                page = order.pop()
+            else:
+                n = min(n, j * block)
+                break
+            tables[b][j] = page
+            if 0 <= page < blocks:
+                counts[page] += 1
+        lens.append(n)
+    if odd:
+        lens[r.randrange(seqs)] = r.choice([-3, width * block + 5])
+        counts = [c if c else r.choice([0, 0, -1, -7]) for c in counts]
+    return tables, lens, counts
+
+
+def _dev(dev, *lists):
+    return [torch.tensor(x, dtype=I, device=dev) for x in lists]
+
+
+POOLS = [(1, 16, 1, 1), (7, 16, 3, 3), (64, 16, 9, 12), (300, 32, 40, 9), (8192, 8, 200, 33), (8193, 16, 33, 40), (20000, 1, 65, 200)]
+
+
+@pytest.mark.parametrize("row,block,blocks,layers,pairs", [(64, 16, 9, 1, 3), (48, 7, 33, 2, 16), (1024, 128, 24, 3, 11), (16, 1, 5, 1, 2)])
+def test_copy(paged, dev, row, block, blocks, layers, pairs):
+    caches = _caches(dev, blocks, row, block, layers)
+    order = torch.randperm(blocks)[: 2 * pairs].tolist()
+    src, dst = order[:pairs] + [-1, blocks, 0, 1], order[pairs:2 * pairs] + [0, 1, blocks, -5]
+    want = [c.clone() for c in caches]
+    for s, d in zip(src, dst):
+        if 0 <= s < blocks and 0 <= d < blocks:
+            for w, c in zip(want, caches):
+                w[d] = c[s]
+    s, d = _dev(dev, src, dst)
+    assert paged.copy_pages(caches[:layers], caches[layers:], s, d) is None
+    assert all(_same_bits(a, b) for a, b in zip(caches, want))
+    paged.copy_pages(caches[:layers], caches[layers:], s[:0], d[:0])
+    paged.copy_pages(caches[:layers], [], s[-4:], d[-4:])
+    assert all(_same_bits(a, b) for a, b in zip(caches, want))
+
+
+@pytest.mark.parametrize("blocks,block,seqs,width", POOLS)
+@pytest.mark.parametrize("children", [1, 5, 70])
+def test_fork(paged, dev, blocks, block, seqs, width, children):
+    for seed in range(3):
+        tables, lens, counts = _pool(seed, blocks, block, seqs, width)
+        r = random.Random(seed + 99)
+        parents = [r.randrange(-1, seqs + 1) for _ in range(children)]
+        if seed == 2:  # a pool that is nearly full
+            counts = [c if r.random() < 4 / blocks or c > 0 else 1 for c in counts]
+        caches = _caches(dev, blocks, 32, block, 2, seed)
+        ref = S.PoolRef(counts, block)
+        rows, out_lens = ref.fork(tables, lens, parents)
+        t, l, p, c = _dev(dev, tables, lens, parents, counts)
+        keep = [x.clone() for x in (t, l, p, c)]
+        want = [ref.moved(x.cpu()) for x in caches]
+        got = paged.fork_sequences(t, l, p, c, caches[:2], caches[2:])
+        assert got[0].tolist() == rows and got[1].tolist() == out_lens and got[2].tolist() == ref.counts
+        assert all(_same_bits(a, b) for a, b in zip(caches, want))
+        assert all(torch.equal(a, b) for a, b in zip(keep, (t, l, p, c)))
+
+
+@pytest.mark.parametrize("blocks,block,seqs,width", POOLS)
+def test_extend(paged, dev, blocks, block, seqs, width):
+    for seed in range(4):
+        tables, lens, counts = _pool(seed + 10, blocks, block, seqs, width)
+        r = random.Random(seed + 5)
+        wanted = [r.choice([n + 1, n, 0, -1, width * block, width * block + 1, 2 ** 31 - 1, n + r.randrange(3 * block)]) for n in lens]
+        ref = S.PoolRef(counts, block)
+        rows, granted = ref.extend(tables, lens, wanted)
+        t, l, w, c = _dev(dev, tables, lens, wanted, counts)
+        got = paged.extend_sequences(t, l, w, c, block)
+        assert got[0].tolist() == rows and got[1].tolist() == granted and got[2].tolist() == ref.counts
+        assert t.tolist() == tables and c.tolist() == counts
+
+
+@pytest.mark.parametrize("blocks,block,seqs,width", POOLS)
+def test_free(paged, dev, blocks, block, seqs, width):
+    for seed in range(3):
+        tables, lens, counts = _pool(seed + 20, blocks, block, seqs, width)
+        r = random.Random(seed)
+        which = [r.randrange(-2, seqs + 2) for _ in range(r.choice([0, 1, seqs, 3 * seqs]))]  # the same one several times too
+        ref = S.PoolRef(counts, block)
+        ref.free(tables, lens, which)
+        t, l, w, c = _dev(dev, tables, lens, which, counts)
+        assert paged.free_sequences(t, l, w, c, block).tolist() == ref.counts
+        assert c.tolist() == counts
+
+
+@pytest.mark.parametrize("blocks,block,seqs,width", POOLS)
+def test_compact(paged, dev, blocks, block, seqs, width):
+    for seed in range(3):
+        tables, lens, counts = _pool(seed + 30, blocks, block, seqs, width)
+        if seed == 1:
+            counts = [max(c, 1) for c in counts]  # nothing free
+        if seed == 2:
+            counts = [0] * blocks                 # nothing used
+        ref = S.PoolRef(counts, block)
+        rows, used = ref.compact(tables, lens)
+        caches = _caches(dev, blocks, 48, block, 1, seed)
+        want = [ref.moved(x.cpu()) for x in caches]
+        t, l, c = _dev(dev, tables, lens, counts)
+        got = paged.compact_pages(t, l, c, caches[:1], caches[1:])
+        assert got[0].tolist() == rows and got[1].tolist() == ref.counts and got[2].tolist() == [used]
+        assert all(_same_bits(a, b) for a, b in zip(caches, want))
+        assert t.tolist() == tables and c.tolist() == counts
+
+
+def test_many_layers_and_pages_larger_than_a_copy_step(paged, dev):
+    blocks, block, row = 12, 160, 1024
+    caches = _caches(dev, blocks, row, block, 3)
+    tables, lens, counts = [[4, 9], [7, 2]], [159, 201], [0] * blocks
+    for row_, n in zip(tables, lens):
+        for j in range(-(-n // block)):
+            counts[row_[j]] = 1
+    ref = S.PoolRef(counts, block)
+    rows, out = ref.fork(tables, lens, [1, 0, 1])
+    want = [ref.moved(x.cpu()) for x in caches]
+    t, l, p, c = _dev(dev, tables, lens, [1, 0, 1], counts)
+    got = paged.fork_sequences(t, l, p, c, caches[:3], caches[3:])
+    assert got[0].tolist() == rows and got[1].tolist() == out
+    assert all(_same_bits(a, b) for a, b in zip(caches, want))
+
+
+def test_a_beam_step_in_a_graph(paged, dev):
+    """Fork, extend, free and pack captured once, on one stream, and replayed on pools that change in place."""
+    blocks, block, seqs, width = 60, 16, 5, 8
+    state = _dev(dev, *_pool(0, blocks, block, seqs, width, odd=False))
+    parents, rows_all = _dev(dev, [0, 0, 3, 1], list(range(seqs)))
+    caches = _caches(dev, blocks, 32, block, 1)
+    start = [x.clone() for x in caches]
+    wanted = torch.zeros(4, dtype=I, device=dev)
+
+    def step():
+        rows, lens, counts = paged.fork_sequences(*state[:2], parents, state[2], caches[:1], caches[1:])
+        room, granted, counts = paged.extend_sequences(rows, lens, wanted, counts, block)
+        counts = paged.free_sequences(*state[:2], rows_all, counts, block)
+        return [rows, lens, room, granted, *paged.compact_pages(room, granted, counts, caches[:1], caches[1:])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in range(5):
+        tables, lens, counts = _pool(seed, blocks, block, seqs, width, odd=False)
+        for s, v in zip(state, (tables, lens, counts)):
+            s.copy_(torch.tensor(v, dtype=I))
+        wanted.copy_(torch.tensor([lens[p] + 1 for p in (0, 0, 3, 1)], dtype=I))
+        for x, y in zip(caches, start):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in held]
+        after = [x.clone() for x in caches]
+        for x, y in zip(caches, start):
+            x.copy_(y)
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+        assert all(_same_bits(a, b) for a, b in zip(after, caches))
+        ref = S.PoolRef(counts, block)
+        rows, out = ref.fork(tables, lens, [0, 0, 3, 1])
+        room, granted = ref.extend(rows, out, wanted.tolist())
+        ref.free(tables, lens, range(seqs))
+        first, ref.moves = ref.moved(start[0].cpu()), []
+        packed, used = ref.compact(room, granted)
+        assert [x.tolist() for x in got] == [rows, out, room, granted, packed, ref.counts, [used]]
+        assert _same_bits(after[0], ref.moved(first))
