@@ -11,13 +11,41 @@ lowest first in the order of the requests, so a host that keeps a copy of the st
 ``[num_blocks, kv_heads*D/16, block_size, 16]``."""
 from __future__ import annotations
 
-from typing import Sequence
+from typing import Optional, Sequence
 
 import torch
 
 import ascend910a_extras.ascend910a_extras_C as _C
 
 Tensor = torch.Tensor
+
+
+def paged_attention_chunk(
+    q: Tensor,
+    key_cache: Tensor,
+    value_cache: Tensor,
+    block_tables: Tensor,
+    context_lens: Tensor,
+    query_starts: Tensor,
+    scale: Optional[float] = None,
+    window: int = 0,
+    return_lse: bool = False,
+    out: Optional[Tensor] = None,
+):
+    """Attention of any number of new tokens per sequence over the paged caches, which hold their K and V already
+    (``ops.reshape_and_cache``): prompts, chunks of prompts, drafted tokens and single tokens in one batch.
+
+    ``q [tokens, heads, D]`` holds the new tokens of all sequences one after the other; sequence ``b`` has the rows
+    ``query_starts[b]:query_starts[b+1]`` (int32 ``[sequences + 1]``), which are the last tokens of its ``context_lens[b]``.  A
+    row sees the keys up to its own position, only the last ``window`` of them where ``window > 0``; kv head and page of a key
+    as in ``ops.paged_attention``, ``scale`` 1/sqrt(D) if not given.  A row that sees nothing (a context shorter than the new
+    tokens) is 0.  Lengths and tables are read on the device only.
+
+    Returns ``o`` like ``q``, with ``return_lse`` also the natural log-sum-exp of the scaled scores, fp32 ``[tokens, heads]``
+    (-inf where nothing is seen), by which results over parts of a context can be joined.  Rows of no sequence (a batch padded
+    behind ``query_starts[-1]``) are not written: they keep what ``out`` held, if that is given, and are undefined if not."""
+    return _C.paged_attention_chunk(q, key_cache, value_cache, block_tables, context_lens, query_starts, scale, window,
+                                    return_lse, out)
 
 
 def copy_pages(key_caches: Sequence[Tensor], value_caches: Sequence[Tensor], src_pages: Tensor, dst_pages: Tensor) -> None:

@@ -35,6 +35,11 @@ SOURCES = [
     "moe.hip",
     "reshape_and_cache.hip",
     "paged_attention.hip",
+    "paged_attention_chunk.hip",
+    "paged_attention_chunk_d0.hip",
+    "paged_attention_chunk_d1.hip",
+    "paged_attention_chunk_d2.hip",
+    "paged_attention_chunk_d3.hip",
     "grouped_matmul.hip",
     "grouped_matmul_tiles.hip",
     "grouped_matmul_persistent.hip",

@@ -17,6 +17,7 @@
 #include <pybind11/stl.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <cmath>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -71,6 +72,8 @@ void* dev_ptr(const Tensor& t) {
 }
 
 void* dev_ptr(const std::optional<Tensor>& t) { return t.has_value() ? dev_ptr(*t) : nullptr; }
+const int32_t* ints(const Tensor& t) { return static_cast<const int32_t*>(dev_ptr(t)); }
+int32_t* ints_out(const Tensor& t) { return static_cast<int32_t*>(dev_ptr(t)); }
 
 // Makes the tensors' device current for the call and hands out torch's current stream on it.
 struct Launch {
@@ -466,6 +469,70 @@ py::object rope_reshape_and_cache(const Tensor& q, const Tensor& k, const Tensor
   return py::cast(out_q);
 }
 
+// ---- attention of a chunk of new tokens ------------------------------------------------------------
+
+py::object paged_attention_chunk(const Tensor& q, const Tensor& key_cache, const Tensor& value_cache,
+                                 const Tensor& block_tables, const Tensor& context_lens, const Tensor& query_starts,
+                                 std::optional<double> scale, int64_t window, bool return_lse,
+                                 const std::optional<Tensor>& out) {
+  const char* name = "paged_attention_chunk";
+  TORCH_CHECK(q.dim() == 3 && key_cache.dim() == 4 && value_cache.dim() == 4 && block_tables.dim() == 2 &&
+                  context_lens.dim() == 1 && query_starts.dim() == 1,
+              name, ": q must be 3D, key_cache and value_cache 4D, block_tables 2D, context_lens and query_starts 1D");
+  TORCH_CHECK(q.is_contiguous() && key_cache.is_contiguous() && value_cache.is_contiguous() &&
+                  block_tables.is_contiguous() && context_lens.is_contiguous() && query_starts.is_contiguous(),
+              name, ": all input tensors must be contiguous");
+  const int64_t tokens = q.size(0), num_heads = q.size(1), head_dim = q.size(2), seqs = block_tables.size(0);
+  const int64_t num_blocks = key_cache.size(0), nh16 = key_cache.size(1), block_size = key_cache.size(2);
+  TORCH_CHECK(key_cache.size(3) == 16, name, ": last dimension of the caches must be 16, got ", key_cache.size(3));
+  TORCH_CHECK(value_cache.sizes() == key_cache.sizes(), name, ": key_cache and value_cache must have the same shape");
+  TORCH_CHECK(head_dim > 0 && head_dim <= 256 && head_dim % 16 == 0, name,
+              ": head_dim must be a multiple of 16 up to 256, got ", head_dim);
+  TORCH_CHECK(nh16 > 0 && (nh16 * 16) % head_dim == 0, name, ": cache rows (", nh16 * 16, " halfs) must hold whole heads of ",
+              head_dim);
+  const int64_t num_kv_heads = nh16 * 16 / head_dim;
+  TORCH_CHECK(num_heads > 0 && num_heads % num_kv_heads == 0, name, ": num_heads (", num_heads,
+              ") must be a multiple of num_kv_heads (", num_kv_heads, ")");
+  TORCH_CHECK(block_size > 0, name, ": the caches' pages must have tokens");
+  TORCH_CHECK(context_lens.size(0) == seqs, name, ": context_lens must have one entry per row of block_tables");
+  TORCH_CHECK(query_starts.size(0) == seqs + 1, name, ": query_starts must have one entry more than block_tables has rows, got ",
+              query_starts.size(0), " and ", seqs);
+  const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)head_dim);
+  TORCH_CHECK(std::isfinite((float)s) && (float)s > 0.f, name, ": scale must be positive and finite, got ", s);
+  TORCH_CHECK(window >= 0, name, ": window must not be negative, got ", window);
+  require_device(name, {{"q", q, at::kHalf},
+                        {"key_cache", key_cache, at::kHalf},
+                        {"value_cache", value_cache, at::kHalf},
+                        {"block_tables", block_tables, at::kInt},
+                        {"context_lens", context_lens, at::kInt},
+                        {"query_starts", query_starts, at::kInt}});
+  if (out.has_value()) {
+    TORCH_CHECK(out->sizes() == q.sizes() && out->is_contiguous(), name, ": out must be contiguous with the shape of q");
+    require_device(name, {{"q", q, at::kHalf}, {"out", *out, at::kHalf}});
+    const auto bytes = [](const Tensor& t) { return std::make_pair((uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + t.nbytes()); };
+    for (const Tensor* t : {&q, &key_cache, &value_cache})
+      TORCH_CHECK(bytes(*out).second <= bytes(*t).first || bytes(*t).second <= bytes(*out).first, name,
+                  ": out must not overlap q or the caches");
+  }
+  Tensor o = out.has_value() ? *out : fresh_like(q);
+  Tensor lse;
+  if (return_lse) lse = fresh(q, {tokens, num_heads}, at::kFloat);
+  if (tokens > 0 && seqs > 0) {
+    Launch l(q);
+    const size_t ws_bytes = aops_paged_attention_chunk_workspace(tokens, seqs, num_heads, num_kv_heads, head_dim, block_size,
+                                                                 block_tables.size(1));
+    TORCH_CHECK(ws_bytes > 0, name, ": unsupported size");
+    Tensor ws = scratch(q, ws_bytes);
+    status(name, aops_paged_attention_chunk_f16(dev_ptr(q), dev_ptr(key_cache), dev_ptr(value_cache), ints(block_tables),
+                                                ints(context_lens), ints(query_starts), dev_ptr(o),
+                                                return_lse ? static_cast<float*>(dev_ptr(lse)) : nullptr, (float)s, window,
+                                                ws.data_ptr(), ws_bytes, tokens, seqs, num_heads, num_kv_heads, head_dim,
+                                                block_size, block_tables.size(1), num_blocks, l.stream));
+  }
+  if (return_lse) return py::cast(std::make_tuple(o, lse));
+  return py::cast(o);
+}
+
 // ---- rotary positions ------------------------------------------------------------------------------
 
 std::tuple<Tensor, Tensor> rotary_tables(int64_t max_position, int64_t rotary_dim, double base, int64_t scaling,
@@ -582,9 +649,6 @@ void require_ints(const char* name, const Tensor* with, std::initializer_list<In
     TORCH_CHECK(a.t.device() == with->device(), name, ": all tensors must be on the same device");
   }
 }
-
-const int32_t* ints(const Tensor& t) { return static_cast<const int32_t*>(dev_ptr(t)); }
-int32_t* ints_out(const Tensor& t) { return static_cast<int32_t*>(dev_ptr(t)); }
 
 void copy_pages(const std::vector<Tensor>& key_caches, const std::vector<Tensor>& value_caches, const Tensor& src_pages,
                 const Tensor& dst_pages) {
@@ -765,6 +829,9 @@ PYBIND11_MODULE(ascend910a_extras_C, m) {
         py::arg("position_ids"), py::arg("cos_cache"), py::arg("sin_cache"), py::arg("key_cache"),
         py::arg("value_cache"), py::arg("slot_indices"), py::arg("return_k") = false,
         py::arg("q_norm_weight") = py::none(), py::arg("k_norm_weight") = py::none(), py::arg("epsilon") = 1e-6);
+  m.def("paged_attention_chunk", &paged_attention_chunk, py::arg("q"), py::arg("key_cache"), py::arg("value_cache"),
+        py::arg("block_tables"), py::arg("context_lens"), py::arg("query_starts"), py::arg("scale"), py::arg("window"),
+        py::arg("return_lse"), py::arg("out"));
   m.def("rotary_tables", &rotary_tables, py::arg("max_position"), py::arg("rotary_dim"), py::arg("base"),
         py::arg("scaling"), py::arg("factor"), py::arg("original_max_position"), py::arg("low"), py::arg("high"),
         py::arg("attention_factor"), py::arg("pair_factors"), py::arg("fp32"), py::arg("device"));

@@ -1,0 +1,829 @@
+// Attention of a chunk of new tokens per sequence over the [num_blocks, Hkv*D/16, block_size, 16] fp16 caches: the kernel,
+// a template over head_dim.
+//
+//   row (token i, head h) of sequence b sits at position p = L_b - n_b + i and sees keys max(0, p - window + 1) .. p:
+//   o = sum_j softmax_j(scale q.k_j) v_j,   lse = log sum_j exp(scale q.k_j)
+//
+// Work.  The query heads of a kv head share its K and V, so a kv head's rows are (token, head of the group) pairs, token
+// by token, and a tile is up to 256 of them (head_dim above 128: 128) from one sequence.  A workgroup of eight (four) waves,
+// one per CU, runs over the keys a tile sees, once, with the running maximum and sum of its softmax in registers.
+//
+//  * More than 32 rows ("tile"): wave w owns rows 32w .. 32w+31, in two blocks of 16 columns; the waves
+//    share K and V tiles of kTile tokens in LDS, double buffered, the next one on its way through registers while this one
+//    is computed.
+//  * Fewer ("stream", the decode-like case): every wave owns all rows and its own 32 tokens of every 256 (128); K goes from
+//    memory straight into the operand registers, V through the wave's own piece of LDS, no barriers in the loop, and the
+//    eight waves are joined through LDS at the end.
+//
+// Operands.  The cache layout is the operand layout of v_mfma_f32_16x16x32_f16: lane (n = lane%16, kg = lane/16) takes for
+// token n the 16 bytes that hold d = 32s + 8kg ..+7, so S^T[token][row] = K . Q^T needs no shuffling, in LDS or out of it (a
+// tile keeps the cache's [chunk of 16 d][token][16], and every fragment read covers contiguous bytes).  S^T leaves lane
+// (row n, kg) with tokens 4kg ..+3 of each group of 16; two groups packed to fp16 are the operand P^T of O^T += V^T . P^T, with
+// the 32 tokens of a step in the order 16g + 4kg + i.  V^T in that order is what ds_read_b64_tr_b16 returns from the same
+// layout: 16 lanes read 4 tokens x 16 d, 128 contiguous bytes, and lane n receives d = n of the four.
+//
+// Softmax.  In log2 units, fp32.  The reference value of a row moves only when the maximum has grown by more than
+// 2^kSlack over it, so accumulators are rarely rescaled; weights are exp2(s - ref + kLift), which keeps those up to 2^-20 of
+// the largest normal numbers when they are rounded to fp16 for the product, at most 2^(kLift + kSlack) = 2^14.  Their sum is
+// taken before that rounding.
+//
+// Masked places.  Scores out of sight are replaced, not added to, so their K may hold anything.  V rows behind the context
+// are zeroed on the way in; a V row that some rows of the tile see and others must not, and that holds an infinity or NaN,
+// would spread through the product as 0 * inf, so tiles at an edge of the mask are searched for such values and, where
+// there are any, take a product that keeps them apart (chunk_pv_guarded).
+#pragma once
+
+#include "aops_common.h"
+
+namespace aops {
+
+// Waves of a workgroup, 32 rows of a tile each: eight with 256 registers, or, for heads whose accumulators and operands take
+// more, four with 512.
+__host__ __device__ constexpr int chunk_waves(int head_dim) { return head_dim <= 128 ? 8 : 4; }
+__host__ __device__ constexpr int chunk_rows(int head_dim) { return 32 * chunk_waves(head_dim); }
+constexpr int kChunkUnit = 256;    // tokens per unit of the balanced partition
+constexpr int kChunkMaxTiles = 2048;  // of the balanced partition
+constexpr float kChunkNegBig = -1.0e30f;
+constexpr float kChunkLog2e = 1.4426950408889634f;
+constexpr float kChunkLn2 = 0.6931471805599453f;
+constexpr float kChunkLift = 6.0f, kChunkSlack = 8.0f;
+
+struct ChunkArgs {
+  const f16 *q, *key_cache, *value_cache;
+  const int32_t *block_tables, *context_lens, *query_starts;
+  f16* out;
+  float* lse;            // may be null
+  float *part_o, *part_ml;  // partial results: [kv head][2 * shares][part_rows][D] and [..][2]
+  int32_t* plan;         // units in front of each tile (max_tiles + 1), sequence and number of each tile
+  int32_t tokens, seqs, num_heads, num_kv_heads, group, block_size, max_pages, num_blocks, window;
+  int32_t max_tiles, tile_rows, shares, part_rows;  // shares: of the balanced partition, per kv head; 0: one workgroup per tile
+  uint32_t block_magic, block_shift;  // x / block_size = x * magic >> shift, x < 2^31
+  float scale_log2;
+};
+
+// A tile: rows row0 .. row0 + rows - 1 of sequence b's (token, head) rows.
+struct ChunkTile {
+  int b, q0, row0, rows;
+  int p_first, p_last;  // positions of its first and last row's tokens (may be negative: sees nothing)
+  int ctx;              // keys there are
+  int lo, hi;           // keys seen by any of its rows
+  int unit0, units;     // in units of kChunkUnit tokens, at least one
+};
+
+__device__ __forceinline__ void chunk_seq(const ChunkArgs& a, int b, int& q0, int& n) {
+  q0 = min(max(a.query_starts[b], 0), a.tokens);
+  n = min(max(a.query_starts[b + 1], q0), a.tokens) - q0;
+}
+
+__device__ __forceinline__ int chunk_tiles(const ChunkArgs& a, int n) {
+  return (n * a.group + a.tile_rows - 1) / a.tile_rows;
+}
+
+// First key that the row at position p sees through the window (a row at a negative position sees nothing anyway).
+__device__ __forceinline__ int chunk_window_start(int p, int window) { return max(p, 0) - window + 1; }
+
+__device__ __forceinline__ ChunkTile chunk_geometry(const ChunkArgs& a, int b, int index) {
+  ChunkTile t;
+  int n;
+  t.b = b;
+  chunk_seq(a, b, t.q0, n);
+  t.row0 = index * a.tile_rows;
+  t.rows = min(n * a.group - t.row0, a.tile_rows);
+  const int len = max(a.context_lens[b], 0);
+  t.ctx = (int)min((int64_t)len, (int64_t)a.max_pages * a.block_size);
+  t.p_first = len - n + t.row0 / a.group;
+  t.p_last = len - n + (t.row0 + t.rows - 1) / a.group;
+  t.lo = a.window > 0 ? min(max(chunk_window_start(t.p_first, a.window), 0), t.ctx) : 0;
+  t.hi = min(max(t.p_last + 1, 0), t.ctx);
+  t.unit0 = t.lo / kChunkUnit;
+  t.units = max((t.hi - 1) / kChunkUnit + 1 - t.unit0, 1);
+  return t;
+}
+
+// How a head of D elements is cut up for the matrix core.
+template <int D>
+struct ChunkDims {
+  static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head_dim: a multiple of 16 up to 256");
+  static constexpr int kFull = D / 32;         // slices of 32 d of the score product
+  static constexpr int kTail = (D % 32) / 16;  // and a half slice: 16 d in the lanes kg < 2, zeros in the others, in Q and K
+  static constexpr int kSlices = kFull + kTail;
+  static constexpr int kBlocks = D / 16;       // chunks of the cache, blocks of 16 d of O^T
+  static constexpr int kWaves = chunk_waves(D), kThreads = kWaves * kWave;
+  static constexpr int kTile = D <= 192 ? 64 : 32;        // tokens of a shared tile: what the registers leave room for
+  static constexpr int kStreamBlocks = 2;                 // column blocks of the stream path
+  static constexpr int kLds = 4 * kTile * D * 2;          // two buffers of K and V
+  static constexpr int kStreamLds = kWaves * 32 * D * 2;
+  static constexpr int kJoinBlocks = 4;                   // blocks of O^T joined at a time: 64 KiB of LDS, or 32
+  static constexpr int kJoinLds = kWaves * 16 * kStreamBlocks * kJoinBlocks * 16 * 4;
+  static constexpr int kMain = kLds > kStreamLds ? (kLds > kJoinLds ? kLds : kJoinLds) : (kStreamLds > kJoinLds ? kStreamLds : kJoinLds);
+  static constexpr int kSmall = 2 * kWaves * 32 * 4 + 16;         // joined maxima and sums, flags
+  static constexpr int kPlan = (3 * kChunkMaxTiles + 1) * 4;
+};
+
+typedef __fp16 ChunkTr __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) ChunkTr ChunkTrLds;
+
+__device__ __forceinline__ f16x4 chunk_read_tr(const f16* lds) {
+  return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((ChunkTrLds*)lds));
+}
+
+// Largest of the four lanes n, n + 16, n + 32, n + 48, in all four.  (The swaps exchange halves and quarters of the wave
+// between two registers; written as assembly because the compiler folds the builtins' two results into one when both
+// operands are the same value.  Their two wait states are part of it.)
+__device__ __forceinline__ float chunk_max4(float x) {
+  float y = x;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  x = fmaxf(x, y);
+  y = x;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  return fmaxf(x, y);
+}
+__device__ __forceinline__ float chunk_sum4(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+__device__ __forceinline__ bool chunk_not_finite(f16x8 v) {
+  const u32x4 u = __builtin_bit_cast(u32x4, v);
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    bad |= (u[i] & 0x7c00u) == 0x7c00u;
+    bad |= (u[i] & 0x7c000000u) == 0x7c000000u;
+  }
+  return bad;
+}
+
+// Offset (in halfs) of token tok of the tile's sequence, from the start of the cache's kv head 0; entries outside the cache
+// read the nearest page.
+__device__ __forceinline__ int64_t chunk_token_offset(const ChunkArgs& a, const int32_t* table, int tok, int64_t page_elems) {
+  const int blk = (int)((uint64_t)(uint32_t)tok * a.block_magic >> a.block_shift);  // tok / block_size
+  const int page = min(max(table[blk], 0), a.num_blocks - 1);
+  return page * page_elems + (int64_t)(tok - blk * a.block_size) * 16;
+}
+
+template <int D, int CB>
+struct ChunkState {
+  f32x4 o[CB][ChunkDims<D>::kBlocks];  // O^T: lane (row n, kg), element i <-> d = 16 block + 4kg + i
+  float ref[CB];                       // reference value of the row's weights, log2 units
+  float sum[CB];                       // this lane's share of the sum of weights
+};
+
+template <int D, int CB>
+struct ChunkQuery {
+  f16x8 d[CB][ChunkDims<D>::kSlices];
+  int pos[CB];  // position of this lane's row; a row that is none: -1
+};
+
+template <int D, int CB>
+__device__ __forceinline__ void chunk_load_query(const ChunkArgs& a, const ChunkTile& t, int head, int first_row, int n, int kg,
+                                                 ChunkQuery<D, CB>& q) {
+  using Dims = ChunkDims<D>;
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+    const int r = first_row + 16 * c + n;
+    const bool live = r < t.rows;
+    const int row = t.row0 + (live ? r : 0);
+    const int token = row / a.group;
+    q.pos[c] = live ? t.p_first + token - t.row0 / a.group : -1;
+    const f16* src = a.q + ((int64_t)(t.q0 + token) * a.num_heads + head * a.group + (row - token * a.group)) * D;
+    const f16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < Dims::kSlices; ++s) {
+      q.d[c][s] = zero8;
+      if (live && (s < Dims::kFull || kg < 2)) q.d[c][s] = ld128(src + 32 * s + 8 * kg);
+    }
+  }
+}
+
+template <int D, int CB>
+__device__ __forceinline__ void chunk_init(ChunkState<D, CB>& st) {
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+#pragma unroll
+    for (int db = 0; db < ChunkDims<D>::kBlocks; ++db) st.o[c][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    st.ref[c] = kChunkNegBig;
+    st.sum[c] = 0.f;
+  }
+}
+
+// Scores out of sight become -inf.  Lane (row n, kg) has tokens token0 + 16g + 4kg + i.
+template <int CB, int KG>
+__device__ __forceinline__ void chunk_mask(float (&s)[CB][KG][4], const int (&pos)[CB], int token0, int ctx, int window, int kg) {
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+    const int last = min(pos[c], ctx - 1);
+    const int first = window > 0 ? pos[c] - window + 1 : 0;
+#pragma unroll
+    for (int g = 0; g < KG; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = token0 + 16 * g + 4 * kg + i;
+        if (tok > last || tok < first) s[c][g][i] = -__builtin_inff();
+      }
+  }
+}
+
+// Online softmax; leaves the weights in s (fp32) and returns them packed as P^T operands of 32 tokens each.
+template <int D, int CB, int KG>
+__device__ __forceinline__ void chunk_softmax(float (&s)[CB][KG][4], ChunkState<D, CB>& st, f16x8 (&p)[CB][KG / 2]) {
+  float top[CB];
+  bool moved = false;
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+    float m = s[c][0][0];
+#pragma unroll
+    for (int g = 0; g < KG; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = fmaxf(m, s[c][g][i]);
+    top[c] = chunk_max4(m);
+    moved |= top[c] > st.ref[c] + kChunkSlack;
+  }
+  if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      const float ref = fmaxf(st.ref[c], top[c]);
+      const float alpha = __builtin_amdgcn_exp2f(st.ref[c] - ref);
+      st.ref[c] = ref;
+      st.sum[c] *= alpha;
+#pragma unroll
+      for (int db = 0; db < ChunkDims<D>::kBlocks; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[c][db][i] *= alpha;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+    const float base = kChunkLift - st.ref[c];
+    float sum = 0.f;
+#pragma unroll
+    for (int g = 0; g < KG; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = __builtin_amdgcn_exp2f(s[c][g][i] + base);
+        s[c][g][i] = w;
+        sum += w;
+      }
+    st.sum[c] += sum;
+#pragma unroll
+    for (int h = 0; h < KG / 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[c][h][i] = (f16)s[c][2 * h][i];
+        p[c][h][4 + i] = (f16)s[c][2 * h + 1][i];
+      }
+  }
+}
+
+// O^T += V^T . P^T for 16 * KG tokens of a V tile in LDS whose chunks are `stride` halfs apart; v: this wave's first token.
+template <int D, int CB, int KG>
+__device__ __forceinline__ void chunk_pv(const f16* v, int stride, int lane, const f16x8 (&p)[CB][KG / 2], ChunkState<D, CB>& st) {
+#pragma unroll
+  for (int h = 0; h < KG / 2; ++h)
+#pragma unroll
+    for (int db = 0; db < ChunkDims<D>::kBlocks; ++db) {
+      const f16* at = v + db * stride + 2 * h * 256 + lane * 4;
+      const f16x4 lo = chunk_read_tr(at), hi = chunk_read_tr(at + 256);
+      const f16x8 vt = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int c = 0; c < CB; ++c) st.o[c][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p[c][h], st.o[c][db], 0, 0, 0);
+    }
+}
+
+// The same for tiles whose V holds infinities or NaN that not every row may see: they are left out of the product, and what
+// a row does see of them is added as itself.  Which rows see any comes from products of indicators.
+template <int D, int CB, int KG>
+__device__ __forceinline__ void chunk_pv_guarded(const f16* v, int stride, int lane, const f16x8 (&p)[CB][KG / 2],
+                                                 const int (&pos)[CB], int token0, int ctx, int window,
+                                                 ChunkState<D, CB>& st) {
+  const int kg = lane >> 4;
+  // keeps the fragment reads, which are those of the ordinary product, from being moved in front of the branch, all at once
+  asm volatile("" : "+v"(lane));
+  const float inf = __builtin_inff();
+  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int h = 0; h < KG / 2; ++h) {
+    f16x8 seen[CB];
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int tok = token0 + 32 * h + 16 * (e / 4) + 4 * kg + e % 4;
+        seen[c][e] = tok <= min(pos[c], ctx - 1) && (window <= 0 || tok > pos[c] - window) ? (f16)1.0f : (f16)0.0f;
+      }
+#pragma unroll
+    for (int db = 0; db < ChunkDims<D>::kBlocks; ++db) {
+      const f16* at = v + db * stride + 2 * h * 256 + lane * 4;
+      const f16x4 lo = chunk_read_tr(at), hi = chunk_read_tr(at + 256);
+      const f16x8 vt = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      f16x8 finite, up, down;  // NaN counts as both infinities
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = (float)vt[e];
+        finite[e] = __builtin_fabsf(x) < inf ? vt[e] : (f16)0.0f;
+        up[e] = x == inf || x != x ? (f16)1.0f : (f16)0.0f;
+        down[e] = x == -inf || x != x ? (f16)1.0f : (f16)0.0f;
+      }
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        const f32x4 ups = __builtin_amdgcn_mfma_f32_16x16x32_f16(up, seen[c], zero4, 0, 0, 0);
+        const f32x4 downs = __builtin_amdgcn_mfma_f32_16x16x32_f16(down, seen[c], zero4, 0, 0, 0);
+        st.o[c][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(finite, p[c][h], st.o[c][db], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (ups[i] > 0.f) st.o[c][db][i] += inf;
+          if (downs[i] > 0.f) st.o[c][db][i] -= inf;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);  // one block at a time: a rare path must not cost the others their registers
+    }
+  }
+}
+
+// Where a row's result goes: the outputs (part < 0) or slot `part` of the partial results.
+template <int D>
+__device__ __forceinline__ int64_t chunk_out_row(const ChunkArgs& a, const ChunkTile& t, int head, int r) {
+  const int row = t.row0 + r, token = row / a.group;
+  return (int64_t)(t.q0 + token) * a.num_heads + head * a.group + (row - token * a.group);
+}
+__device__ __forceinline__ int64_t chunk_part_row(const ChunkArgs& a, int head, int part, int r) {
+  return ((int64_t)head * 2 * a.shares + part) * a.part_rows + r;
+}
+// log-sum-exp (natural) of weights exp2(s - ref + kChunkLift) that add up to sum
+__device__ __forceinline__ float chunk_lse(float ref, float sum) {
+  return sum > 0.f || sum != sum ? (ref - kChunkLift + __builtin_amdgcn_logf(sum)) * kChunkLn2 : -__builtin_inff();
+}
+
+// Keys k0 .. k1-1 (k0 a multiple of the tile) for a tile of many rows.
+template <int D>
+__device__ __forceinline__ void chunk_run_tile(const ChunkArgs& a, const ChunkTile& t, int head, int k0, int k1, int part,
+                                               unsigned char* lds, int* flags) {
+  using Dims = ChunkDims<D>;
+  constexpr int KT = Dims::kTile, KG = KT / 16, CB = 2;
+  constexpr int kPieces = 2 * KT;                       // 16-byte pieces of one chunk of a tile
+  constexpr int kStep = Dims::kThreads / kPieces;       // chunks per round of the workgroup
+  constexpr int kRounds = (Dims::kBlocks + kStep - 1) / kStep;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x & (kWave - 1), n = lane & 15, kg = lane >> 4;
+  const int first_row = 32 * wave;
+  const bool live = first_row < t.rows;
+
+  ChunkQuery<D, CB> q;
+  ChunkState<D, CB> st;
+  chunk_load_query<D, CB>(a, t, head, first_row, n, kg, q);
+  chunk_init<D, CB>(st);
+  const int wp_first = t.p_first + ((t.row0 + first_row) / a.group - t.row0 / a.group);
+  const int wp_last = t.p_first + ((t.row0 + min(first_row + 31, t.rows - 1)) / a.group - t.row0 / a.group);
+
+  const int my_token = (threadIdx.x >> 1) & (KT - 1), my_chunk = threadIdx.x / kPieces;
+  const int64_t page_elems = (int64_t)a.num_kv_heads * D * a.block_size;
+  const int64_t chunk_elems = (int64_t)a.block_size * 16;
+  const int64_t lane_off = (int64_t)head * D * a.block_size + (threadIdx.x & 1) * 8 + my_chunk * chunk_elems;
+  const int32_t* table = a.block_tables + (int64_t)t.b * a.max_pages;
+  f16x8 kreg[kRounds], vreg[kRounds];
+  auto offset_of = [&](int kt) { return chunk_token_offset(a, table, min(kt + my_token, t.ctx - 1), page_elems) + lane_off; };
+  auto load = [&](int64_t off) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+      if ((Dims::kBlocks % kStep == 0) || my_chunk + r * kStep < Dims::kBlocks) {
+        kreg[r] = ld128(a.key_cache + off + r * kStep * chunk_elems);
+        vreg[r] = ld128(a.value_cache + off + r * kStep * chunk_elems);
+      }
+  };
+  // rows that see a tile only in part: behind the first row's position, or in front of the last row's window
+  auto at_edge = [&](int kt, int p_first, int p_last) {
+    return kt + KT - 1 > p_first || kt + KT > t.ctx || (a.window > 0 && kt < chunk_window_start(p_last, a.window));
+  };
+  f16* buffer = reinterpret_cast<f16*>(lds);
+  auto store = [&](int kt, int which) {
+    f16* k = buffer + which * 2 * KT * D + threadIdx.x * 8;
+    f16* v = k + KT * D;
+    const bool beyond = kt + my_token >= t.ctx;
+    bool bad = false;
+    const f16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+      if ((Dims::kBlocks % kStep == 0) || my_chunk + r * kStep < Dims::kBlocks) {
+        if (beyond) vreg[r] = zero8;
+        bad |= chunk_not_finite(vreg[r]);
+        st128(k + r * Dims::kThreads * 8, kreg[r]);
+        st128(v + r * Dims::kThreads * 8, vreg[r]);
+      }
+    if (bad && at_edge(kt, t.p_first, t.p_last)) flags[which] = kt;
+  };
+
+  __syncthreads();  // the last item's reads of LDS are done
+  if (threadIdx.x < 2) flags[threadIdx.x] = -1;
+  __syncthreads();
+  if (k0 < k1) {
+    load(offset_of(k0));
+    store(k0, 0);
+  }
+  int64_t next = k0 + KT < k1 ? offset_of(k0 + KT) : 0;
+  __syncthreads();
+  int which = 0;
+  for (int kt = k0; kt < k1; kt += KT, which ^= 1) {
+    const bool more = kt + KT < k1;
+    if (more) load(next);
+    if (kt + 2 * KT < k1) next = offset_of(kt + 2 * KT);
+    if (live && kt <= wp_last && (a.window <= 0 || kt + KT > chunk_window_start(wp_first, a.window))) {
+      const f16* k = buffer + which * 2 * KT * D;
+      const f16* v = k + KT * D;
+      f32x4 acc[CB][KG];
+      const f16* kfrag = k + (kg >> 1) * KT * 16 + n * 16 + (kg & 1) * 8;
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {
+#pragma unroll
+        for (int c = 0; c < CB; ++c) acc[c][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < Dims::kSlices; ++s) {
+          f16x8 kf;
+          if (s < Dims::kFull) {
+            kf = ld128(kfrag + s * 2 * KT * 16 + g * 256);
+          } else {
+            kf = ld128(k + s * 2 * KT * 16 + g * 256 + n * 16 + (kg & 1) * 8);
+            if (kg >= 2) kf = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+          }
+#pragma unroll
+          for (int c = 0; c < CB; ++c)
+            acc[c][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q.d[c][s], acc[c][g], 0, 0, 0);
+        }
+      }
+      float s[CB][KG][4];
+#pragma unroll
+      for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int g = 0; g < KG; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[c][g][i] = acc[c][g][i] * a.scale_log2;
+      const bool edge = at_edge(kt, wp_first, wp_last);
+      if (edge) chunk_mask<CB, KG>(s, q.pos, kt, t.ctx, a.window, kg);
+      f16x8 p[CB][KG / 2];
+      chunk_softmax<D, CB, KG>(s, st, p);
+      if (edge && flags[which] == kt)
+        chunk_pv_guarded<D, CB, KG>(v, KT * 16, lane, p, q.pos, kt, t.ctx, a.window, st);
+      else
+        chunk_pv<D, CB, KG>(v, KT * 16, lane, p, st);
+    }
+    if (more) store(kt + KT, which ^ 1);
+    __syncthreads();
+  }
+
+  if (!live) return;
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+    const int r = first_row + 16 * c + n;
+    const float sum = chunk_sum4(st.sum[c]);
+    if (r >= t.rows) continue;
+    if (part < 0) {
+      const int64_t row = chunk_out_row<D>(a, t, head, r);
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+      for (int db = 0; db < Dims::kBlocks; ++db) {
+        f16x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (f16)(st.o[c][db][i] * inv);
+        *reinterpret_cast<f16x4*>(a.out + row * D + 16 * db + 4 * kg) = v;
+      }
+      if (a.lse && kg == 0) a.lse[row] = chunk_lse(st.ref[c], sum);
+    } else {
+      const int64_t row = chunk_part_row(a, head, part, r);
+#pragma unroll
+      for (int db = 0; db < Dims::kBlocks; ++db)
+        *reinterpret_cast<f32x4*>(a.part_o + row * D + 16 * db + 4 * kg) = st.o[c][db];
+      if (kg == 0) {
+        a.part_ml[2 * row] = st.ref[c];
+        a.part_ml[2 * row + 1] = sum;
+      }
+    }
+  }
+}
+
+// Keys k0 .. k1-1 (k0 a multiple of the unit) for a tile of at most 16 * kStreamBlocks rows.
+template <int D>
+__device__ __forceinline__ void chunk_run_stream(const ChunkArgs& a, const ChunkTile& t, int head, int k0, int k1, int part,
+                                                 unsigned char* lds, float* small) {
+  using Dims = ChunkDims<D>;
+  constexpr int CB = Dims::kStreamBlocks, KG = 2, kStep = 32 * Dims::kWaves;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x & (kWave - 1), n = lane & 15, kg = lane >> 4;
+  ChunkQuery<D, CB> q;
+  ChunkState<D, CB> st;
+  chunk_load_query<D, CB>(a, t, head, 0, n, kg, q);
+  chunk_init<D, CB>(st);
+  const int64_t page_elems = (int64_t)a.num_kv_heads * D * a.block_size;
+  const int64_t chunk_elems = (int64_t)a.block_size * 16;
+  const int64_t head_off = (int64_t)head * D * a.block_size;
+  const int32_t* table = a.block_tables + (int64_t)t.b * a.max_pages;
+  f16* mine = reinterpret_cast<f16*>(lds) + wave * 32 * D;  // [chunk][32 tokens][16]
+  __syncthreads();  // the last item's reads of LDS are done
+
+  // K operand registers: token n of group g, d = 32s + 8kg ..+7.  V: 16-byte piece `lane` of every chunk's 32 tokens.
+  f16x8 kreg[KG][Dims::kSlices], vreg[Dims::kBlocks];
+  int64_t koff[KG], voff;
+  auto offsets = [&](int token0) {
+#pragma unroll
+    for (int g = 0; g < KG; ++g)
+      koff[g] = chunk_token_offset(a, table, min(token0 + 16 * g + n, t.ctx - 1), page_elems) + head_off;
+    voff = chunk_token_offset(a, table, min(token0 + (lane >> 1), t.ctx - 1), page_elems) + head_off + (lane & 1) * 8;
+  };
+  auto load_k = [&]() {
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+      const f16* src = a.key_cache + koff[g] + (kg >> 1) * chunk_elems + (kg & 1) * 8;
+#pragma unroll
+      for (int s = 0; s < Dims::kSlices; ++s) {
+        if (s < Dims::kFull) {
+          kreg[g][s] = ld128_stream(src + 2 * s * chunk_elems);
+        } else {
+          kreg[g][s] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+          if (kg < 2) kreg[g][s] = ld128_stream(src + 2 * s * chunk_elems);
+        }
+      }
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int db = 0; db < Dims::kBlocks; ++db) vreg[db] = ld128_stream(a.value_cache + voff + db * chunk_elems);
+  };
+  int token0 = k0 + 32 * wave;
+  if (token0 < k1) {
+    offsets(token0);
+    load_k();
+    load_v();
+  }
+  for (; token0 < k1; token0 += kStep) {
+    const bool more = token0 + kStep < k1;
+    if (more) offsets(token0 + kStep);
+    f32x4 acc[CB][KG];
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {
+        acc[c][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < Dims::kSlices; ++s)
+          acc[c][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kreg[g][s], q.d[c][s], acc[c][g], 0, 0, 0);
+      }
+    float s[CB][KG][4];
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+      for (int g = 0; g < KG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[c][g][i] = acc[c][g][i] * a.scale_log2;
+    if (more) load_k();
+    const bool edge = token0 + 31 > t.p_first || token0 + 32 > t.ctx || (a.window > 0 && token0 < chunk_window_start(t.p_last, a.window));
+    bool guarded = false;
+    const f16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (edge) {
+      chunk_mask<CB, KG>(s, q.pos, token0, t.ctx, a.window, kg);
+      bool bad = false;
+#pragma unroll
+      for (int db = 0; db < Dims::kBlocks; ++db) {
+        if (token0 + (lane >> 1) >= t.ctx) vreg[db] = zero8;
+        bad |= chunk_not_finite(vreg[db]);
+      }
+      guarded = __builtin_amdgcn_ballot_w64(bad) != 0;
+    }
+#pragma unroll
+    for (int db = 0; db < Dims::kBlocks; ++db) st128(mine + db * 512 + lane * 8, vreg[db]);
+    if (more) load_v();
+    f16x8 p[CB][KG / 2];
+    chunk_softmax<D, CB, KG>(s, st, p);
+    if (guarded)
+      chunk_pv_guarded<D, CB, KG>(mine, 512, lane, p, q.pos, token0, t.ctx, a.window, st);
+    else
+      chunk_pv<D, CB, KG>(mine, 512, lane, p, st);
+  }
+
+  // Join the waves: common reference and total of every row, then the accumulators, kJoinBlocks blocks of 16 d at a time.
+  float* refs = small;                        // [wave][row]
+  float* sums = small + Dims::kWaves * 32;
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+    const float sum = chunk_sum4(st.sum[c]);
+    if (kg == 0) {
+      refs[wave * 32 + 16 * c + n] = st.ref[c];
+      sums[wave * 32 + 16 * c + n] = sum;
+    }
+  }
+  __syncthreads();
+  float factor[CB];
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+    float ref = kChunkNegBig;
+#pragma unroll
+    for (int w = 0; w < Dims::kWaves; ++w) ref = fmaxf(ref, refs[w * 32 + 16 * c + n]);
+    factor[c] = __builtin_amdgcn_exp2f(st.ref[c] - ref);
+  }
+  float* acc = reinterpret_cast<float*>(lds);  // [wave][row][kJoinBlocks * 16 (+ 4, so that rows start in other banks)]
+  constexpr int kRow = Dims::kJoinBlocks * 16;
+  constexpr int kRowsAt = 16 * CB;
+  for (int db0 = 0; db0 < Dims::kBlocks; db0 += Dims::kJoinBlocks) {
+    __syncthreads();  // LDS is free: V was read, or the blocks in front of these were joined
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+      for (int db = 0; db < Dims::kBlocks; ++db)
+        if (db >= db0 && db < db0 + Dims::kJoinBlocks)
+          *reinterpret_cast<f32x4*>(acc + (wave * kRowsAt + 16 * c + n) * kRow + (db - db0) * 16 + 4 * kg) = st.o[c][db] * factor[c];
+    __syncthreads();
+    const int width = min(Dims::kBlocks - db0, Dims::kJoinBlocks) * 4;  // groups of four d
+    for (int i = threadIdx.x; i < t.rows * width; i += Dims::kThreads) {
+      const int r = i / width, d4 = i - r * width;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      float ref = kChunkNegBig, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < Dims::kWaves; ++w) {
+        v += *reinterpret_cast<const f32x4*>(acc + (w * kRowsAt + r) * kRow + 4 * d4);
+        ref = fmaxf(ref, refs[w * 32 + r]);
+      }
+#pragma unroll
+      for (int w = 0; w < Dims::kWaves; ++w) sum += sums[w * 32 + r] * __builtin_amdgcn_exp2f(refs[w * 32 + r] - ref);
+      const int d = db0 * 16 + 4 * d4;
+      if (part < 0) {
+        const int64_t row = chunk_out_row<D>(a, t, head, r);
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        f16x4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = (f16)(v[j] * inv);
+        *reinterpret_cast<f16x4*>(a.out + row * D + d) = o;
+        if (a.lse && d == 0) a.lse[row] = chunk_lse(ref, sum);
+      } else {
+        const int64_t row = chunk_part_row(a, head, part, r);
+        *reinterpret_cast<f32x4*>(a.part_o + row * D + d) = v;
+        if (d == 0) {
+          a.part_ml[2 * row] = ref;
+          a.part_ml[2 * row + 1] = sum;
+        }
+      }
+    }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void chunk_run(const ChunkArgs& a, const ChunkTile& t, int head, int unit, int units, int part,
+                                          unsigned char* lds, float* small) {
+  const int k0 = (t.unit0 + unit) * kChunkUnit, k1 = min(t.hi, (t.unit0 + unit + units) * kChunkUnit);
+  if (t.rows <= 16 * ChunkDims<D>::kStreamBlocks) {
+    chunk_run_stream<D>(a, t, head, k0, k1, part, lds, small);
+  } else {
+    const int first = max(k0, t.lo / ChunkDims<D>::kTile * ChunkDims<D>::kTile);
+    chunk_run_tile<D>(a, t, head, first, k1, part, lds, reinterpret_cast<int*>(small));
+  }
+}
+
+// Sequence and number of tile `tile` (the same in all lanes), counting the sequences' tiles one after the other; false
+// where there are fewer.
+__device__ __forceinline__ bool chunk_find(const ChunkArgs& a, int tile, int& b, int& index) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int running = 0;
+  for (int64_t base = 0; base < a.seqs; base += kWave) {
+    int q0, n = 0;
+    if (base + lane < a.seqs) chunk_seq(a, (int)base + lane, q0, n);
+    const int mine = chunk_tiles(a, n);
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
+    }
+    const uint64_t behind = __builtin_amdgcn_ballot_w64(running + upto > tile);
+    if (behind) {
+      const int at = __builtin_ctzll(behind);
+      b = (int)base + at;
+      index = tile - running - (__shfl(upto, at) - __shfl(mine, at));
+      b = __builtin_amdgcn_readfirstlane(b);
+      index = __builtin_amdgcn_readfirstlane(index);
+      return true;
+    }
+    running += __shfl(upto, kWave - 1);
+  }
+  return false;
+}
+
+// One workgroup per (tile, kv head), kv heads next to each other so that a kv head's tiles run on one XCD (or few) and share
+// its K and V in that L2.  The last tiles of the sequences, which see the most keys, come first.
+template <int D>
+__global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) void chunk_tiles_kernel(ChunkArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char chunk_lds[];
+  const int head = blockIdx.x % a.num_kv_heads;
+  int b, index;
+  if (!chunk_find(a, a.max_tiles - 1 - (int)(blockIdx.x / a.num_kv_heads), b, index)) return;
+  const ChunkTile t = chunk_geometry(a, b, index);
+  chunk_run<D>(a, t, head, 0, t.units, -1, chunk_lds, reinterpret_cast<float*>(chunk_lds + ChunkDims<D>::kMain));
+}
+
+// Few tiles: their keys, in units of 256 tokens, are laid end to end and cut into `shares` equal shares per kv head.  A tile
+// inside one share is written directly; of the others every share leaves a partial result, in slot 2w of share w if the tile
+// began in front of the share and in slot 2w + 1 if it began in it, which chunk_merge joins in the order of the keys.
+template <int D>
+__global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) void chunk_shares_kernel(ChunkArgs a) {
+  using Dims = ChunkDims<D>;
+  extern __shared__ __attribute__((aligned(16))) unsigned char chunk_lds[];
+  float* small = reinterpret_cast<float*>(chunk_lds + Dims::kMain);
+  int* before = reinterpret_cast<int*>(chunk_lds + Dims::kMain + Dims::kSmall);
+  int* seq = before + kChunkMaxTiles + 1;
+  int* number = seq + kChunkMaxTiles;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int head = blockIdx.x % a.num_kv_heads, share_index = blockIdx.x / a.num_kv_heads;
+  // every thread: the sequence and units of its tiles
+  for (int base = 0; base < a.max_tiles; base += Dims::kThreads) {
+    const int tile = base + threadIdx.x;
+    const int first = __builtin_amdgcn_readfirstlane(tile);  // this wave's 64 tiles
+    int b = -1, index = 0, running = 0;
+    for (int64_t s0 = 0; s0 < a.seqs && running < first + kWave; s0 += kWave) {
+      int q0, n = 0;
+      if (s0 + lane < a.seqs) chunk_seq(a, (int)s0 + lane, q0, n);
+      const int mine = chunk_tiles(a, n);
+      int upto = mine;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+      const int total = __builtin_amdgcn_readlane(upto, kWave - 1);
+      if (running + total > first) {
+        const int lanes = (int)min((int64_t)kWave, a.seqs - s0);
+        for (int k = 0; k < lanes; ++k) {
+          const int end = running + __builtin_amdgcn_readlane(upto, k), begin = end - __builtin_amdgcn_readlane(mine, k);
+          if (tile >= begin && tile < end) {
+            b = (int)s0 + k;
+            index = tile - begin;
+          }
+        }
+      }
+      running += total;
+    }
+    if (tile < a.max_tiles) {
+      seq[tile] = b;
+      number[tile] = index;
+      before[tile + 1] = b >= 0 ? chunk_geometry(a, b, index).units : 0;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < kWave) {  // running sums
+    int running = 0;
+    if (lane == 0) before[0] = 0;
+    for (int base = 0; base < a.max_tiles; base += kWave) {
+      int upto = base + lane < a.max_tiles ? before[base + lane + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+      if (base + lane < a.max_tiles) before[base + lane + 1] = running + upto;
+      running += __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {  // for the join
+    for (int i = threadIdx.x; i <= a.max_tiles; i += Dims::kThreads) a.plan[i] = before[i];
+    for (int i = threadIdx.x; i < a.max_tiles; i += Dims::kThreads) {
+      a.plan[a.max_tiles + 1 + i] = seq[i];
+      a.plan[2 * a.max_tiles + 1 + i] = number[i];
+    }
+  }
+  const int total = before[a.max_tiles];
+  const int share = max((total + a.shares - 1) / a.shares, 1);
+  int begin = (int)min((int64_t)share_index * share, (int64_t)total);
+  const int end = min(begin + share, total);
+  int tile = 0;
+  for (int step = kChunkMaxTiles; step > 0; step >>= 1)  // the last tile that begins at or in front of `begin`
+    if (tile + step < a.max_tiles && before[tile + step] <= begin) tile += step;
+  while (begin < end) {
+    const int from = __builtin_amdgcn_readfirstlane(before[tile]), to = __builtin_amdgcn_readfirstlane(before[tile + 1]);
+    const int upto = min(end, to);
+    const bool whole = begin == from && upto == to;
+    const int part = whole ? -1 : 2 * share_index + (begin == from ? 1 : 0);
+    const ChunkTile t = chunk_geometry(a, __builtin_amdgcn_readfirstlane(seq[tile]), __builtin_amdgcn_readfirstlane(number[tile]));
+    chunk_run<D>(a, t, head, begin - from, upto - begin, part, chunk_lds, small);
+    begin = upto;
+    ++tile;
+  }
+}
+
+typedef hipError_t (*ChunkLaunch)(const ChunkArgs& a, hipStream_t stream);
+
+template <int D>
+hipError_t chunk_launch(const ChunkArgs& a, hipStream_t stream) {
+  using Dims = ChunkDims<D>;
+  static std::atomic<uint64_t> tiles_done{0}, shares_done{0};
+  if (a.shares > 0) {
+    constexpr int lds = Dims::kMain + Dims::kSmall + Dims::kPlan;
+    if (const hipError_t e = allow_dynamic_lds((const void*)chunk_shares_kernel<D>, lds, shares_done)) return e;
+    chunk_shares_kernel<D><<<(unsigned)(a.shares * a.num_kv_heads), Dims::kThreads, lds, stream>>>(a);
+  } else {
+    constexpr int lds = Dims::kMain + Dims::kSmall;
+    if (const hipError_t e = allow_dynamic_lds((const void*)chunk_tiles_kernel<D>, lds, tiles_done)) return e;
+    chunk_tiles_kernel<D><<<(unsigned)((int64_t)a.max_tiles * a.num_kv_heads), Dims::kThreads, lds, stream>>>(a);
+  }
+  return hipGetLastError();
+}
+
+#define AOPS_CHUNK_DIMS(X) \
+  X(16) X(32) X(48) X(64) X(80) X(96) X(112) X(128) X(144) X(160) X(176) X(192) X(208) X(224) X(240) X(256)
+#define AOPS_CHUNK_EXTERN(D) extern template hipError_t chunk_launch<D>(const ChunkArgs&, hipStream_t);
+
+}  // namespace aops

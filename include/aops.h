@@ -126,6 +126,34 @@ int aops_qknorm_rope_reshape_and_cache_f16(
     int64_t head_dim, int64_t num_blocks, int64_t block_size, void* stream);
 
 /*
+ * Attention of a chunk of new tokens per sequence over the paged caches (prompts, chunks of prompts, several drafted
+ * tokens, single tokens, mixed in one batch).  Sequence b has the rows query_starts[b] .. query_starts[b+1] - 1 of q and out
+ * ([tokens, num_heads, head_dim]), n_b of them, which are the LAST n_b tokens of its context of context_lens[b] tokens; their
+ * K and V are in the caches already.  The row of position p = context_lens[b] - n_b + i sees the keys 0 .. p, or with
+ * window > 0 the last `window` of those:
+ *   out = f16( sum_j softmax_j(scale q.k_j) v_j ),   lse = log sum_j exp(scale q.k_j)  (natural logarithm, fp32)
+ * A row that sees nothing (a context shorter than its new tokens) gets out = 0 and lse = -inf.  Rows of no sequence, in front
+ * of query_starts[0] or at and behind query_starts[seqs], are left as they are.
+ * key_cache, value_cache: [num_blocks, num_kv_heads*head_dim/16, block_size, 16]; block_tables: int32 [seqs, max_pages]
+ * (entries outside the cache read the nearest page; keys that no entry of the row holds do not exist); context_lens: int32
+ * [seqs]; query_starts: int32 [seqs + 1], not decreasing (bounds are limited to 0 .. tokens).  lse: fp32
+ * [tokens, num_heads] or NULL.  scale is positive and finite.  What lies in the cache where a row does not see it, infinities
+ * and NaN included, has no effect on it.
+ * head_dim: a multiple of 16 up to 256; num_heads a multiple of num_kv_heads; tokens * num_heads / num_kv_heads below 2^30.
+ * workspace: aops_paged_attention_chunk_workspace bytes (queried with the same device current; 0 = unsupported shape), not
+ * shared with a call that may run at the same time.
+ * No counterpart in the reference, whose attention is decode only (reference csrc/ffi/ops.cpp:408-482).
+ */
+size_t aops_paged_attention_chunk_workspace(int64_t tokens, int64_t seqs, int64_t num_heads, int64_t num_kv_heads,
+                                            int64_t head_dim, int64_t block_size, int64_t max_pages);
+int aops_paged_attention_chunk_f16(const void* q, const void* key_cache, const void* value_cache,
+                                   const int32_t* block_tables, const int32_t* context_lens, const int32_t* query_starts,
+                                   void* out, float* lse, float scale, int64_t window, void* workspace,
+                                   size_t workspace_bytes, int64_t tokens, int64_t seqs, int64_t num_heads,
+                                   int64_t num_kv_heads, int64_t head_dim, int64_t block_size, int64_t max_pages,
+                                   int64_t num_blocks, void* stream);
+
+/*
  * cos and sin tables [max_position, rotary_dim/2] (fp16, or fp32 with table_fp32) of the angles p * f_j,
  * f_j = base^(-2j/rotary_dim), formed in 64 bits; every entry times attention_factor.  rotary_dim is even.
  * scaling changes the frequencies for contexts longer than the model was trained on:

@@ -154,3 +154,45 @@ def test_c_abi_pages():
     for bad in (dict(seqs=-1), dict(width=-1), dict(block=0), dict(rows=-1), dict(blocks=-1), dict(ptr=None)):
         assert free(**bad) == -1, bad
     assert free(blocks=0) == 0
+
+
+def test_chunk_attention_refusals():
+    from ascend910a_extras.paged import paged_attention_chunk as f
+
+    q, c, t, l, s = _half(3, 4, 64), _half(8, 8, 16, 16), _int(2, 4), _int(2), _int(3)
+    _raises(f, q[0], c, c, t, l, s, match="3D")
+    _raises(f, q.transpose(0, 1), c, c, t, l, s, match="contiguous")
+    _raises(f, q, _half(8, 8, 16, 8), _half(8, 8, 16, 8), t, l, s, match="16")
+    _raises(f, q, c, c[:4], t, l, s, match="same shape")
+    _raises(f, _half(3, 4, 72), c, c, t, l, s, match="head_dim")
+    _raises(f, _half(3, 4, 272), c, c, t, l, s, match="head_dim")
+    _raises(f, _half(3, 4, 48), c, c, t, l, s, match="whole heads")
+    _raises(f, _half(3, 5, 64), c, c, t, l, s, match="num_kv_heads")
+    _raises(f, q, c, c, t, _int(3), s, match="context_lens")
+    _raises(f, q, c, c, t, l, l, match="query_starts")
+    _raises(f, q, c, c, t, l, s, scale=-1.0, match="scale")
+    _raises(f, q, c, c, t, l, s, scale=float("inf"), match="scale")
+    _raises(f, q, c, c, t, l, s, window=-1, match="window")
+    _raises(f, q, c, c, t, l, s, match="GPU device")
+
+
+def test_c_abi_chunk_attention():
+    lib = cabi.lib()
+    p = ctypes.c_void_p(16)
+
+    def run(tokens=4, seqs=2, hq=4, hk=2, d=64, block=16, pages=4, blocks=8, scale=0.1, window=0, ptr=p, ws=p, ws_bytes=1 << 30):
+        return lib.aops_paged_attention_chunk_f16(ptr, ptr, ptr, ptr, ptr, ptr, ptr, None, scale, window, ws, ws_bytes, tokens,
+                                                  seqs, hq, hk, d, block, pages, blocks, None)
+
+    assert run(tokens=0) == 0 and run(seqs=0) == 0
+    for bad in (dict(tokens=-1), dict(seqs=-1), dict(hq=0), dict(hk=0), dict(hq=5), dict(d=0), dict(d=72), dict(d=272),
+                dict(block=0), dict(pages=-1), dict(blocks=-1), dict(scale=0.0), dict(scale=float("nan")), dict(window=-1),
+                dict(ptr=None), dict(tokens=1 << 30, hq=4, hk=1), dict(tokens=1 << 31), dict(block=1 << 20, pages=1 << 20)):
+        assert run(**bad) == -1, bad
+    assert run(ws=None) == -2
+    size = lib.aops_paged_attention_chunk_workspace
+    # short tables: no partial results; long ones: two slots per share, rows of the largest tile, and the plan
+    assert size(4, 2, 4, 2, 64, 16, 4) == 16
+    assert size(4, 2, 4, 2, 64, 16, 400) == 2 * 2 * 128 * 16 * 66 * 4 + (3 * 3 + 1) * 4
+    assert run(pages=400, ws_bytes=size(4, 2, 4, 2, 64, 16, 400) - 1) == -2
+    assert size(4, 2, 5, 2, 64, 16, 4) == 0 and size(4, 2, 4, 2, 24, 16, 4) == 0
