@@ -9,8 +9,7 @@
 // one per CU, runs over the keys a tile sees, once, with the running maximum and sum of its softmax in registers.
 //
 //  * More than 32 rows ("tile"): wave w owns rows 32w .. 32w+31, in two blocks of 16 columns; the waves
-//    share K and V tiles of kTile tokens in LDS, double buffered, the next one on its way through registers while this one
-//    is computed.
+//    share K and V tiles of kTile tokens in LDS, which are on their way while others are computed.
 //  * Fewer ("stream", the decode-like case): every wave owns all rows and its own 32 tokens of every 256 (128); K goes from
 //    memory straight into the operand registers, V through the wave's own piece of LDS, no barriers in the loop, and the
 //    eight waves are joined through LDS at the end.
@@ -29,9 +28,11 @@
 //
 // Masked places.  Scores out of sight are replaced, not added to, so their K may hold anything.  V rows behind the context
 // are zeroed on the way in; a V row that some rows of the tile see and others must not, and that holds an infinity or NaN,
-// would spread through the product as 0 * inf, so tiles at an edge of the mask are searched for such values and, where
-// there are any, take a product that keeps them apart (chunk_pv_guarded).
+// would spread through the product as 0 * inf, so tiles at an edge of the mask are searched for such values, which are left out
+// of the products and added to the results (chunk_add_not_finite).
 #pragma once
+
+#include <type_traits>
 
 #include "aops_common.h"
 
@@ -42,7 +43,7 @@ namespace aops {
 __host__ __device__ constexpr int chunk_waves(int head_dim) { return head_dim <= 128 ? 8 : 4; }
 __host__ __device__ constexpr int chunk_rows(int head_dim) { return 32 * chunk_waves(head_dim); }
 constexpr int kChunkUnit = 256;    // tokens per unit of the balanced partition
-constexpr int kChunkMaxTiles = 2048;  // of the balanced partition
+constexpr int kChunkMaxTiles = 1024;  // of the balanced partition
 constexpr float kChunkNegBig = -1.0e30f;
 constexpr float kChunkLog2e = 1.4426950408889634f;
 constexpr float kChunkLn2 = 0.6931471805599453f;
@@ -61,7 +62,18 @@ struct ChunkArgs {
   float scale_log2;
 };
 
-// A tile: rows row0 .. row0 + rows - 1 of sequence b's (token, head) rows.
+// The arguments where the kernel was given them, to be read by scalar loads when they are needed.  chunk_reread: the same, but
+// the compiler does not know, so what the end of a tile needs is not held in registers through its loop.
+typedef const __attribute__((address_space(4))) ChunkArgs ChunkArgsMem;
+typedef ChunkArgsMem& ChunkArgsRef;
+__device__ __forceinline__ ChunkArgsRef chunk_args() { return *(ChunkArgsMem*)__builtin_amdgcn_kernarg_segment_ptr(); }
+__device__ __forceinline__ ChunkArgsRef chunk_reread(ChunkArgsRef a) {
+  ChunkArgsMem* p = &a;
+  asm volatile("" : "+s"(p));
+  return *p;
+}
+
+// A tile: rows row0 + rows - 1 of sequence b's (token, head) rows.
 struct ChunkTile {
   int b, q0, row0, rows;
   int p_first, p_last;  // positions of its first and last row's tokens (may be negative: sees nothing)
@@ -70,19 +82,19 @@ struct ChunkTile {
   int unit0, units;     // in units of kChunkUnit tokens, at least one
 };
 
-__device__ __forceinline__ void chunk_seq(const ChunkArgs& a, int b, int& q0, int& n) {
+__device__ __forceinline__ void chunk_seq(ChunkArgsRef a, int b, int& q0, int& n) {
   q0 = min(max(a.query_starts[b], 0), a.tokens);
   n = min(max(a.query_starts[b + 1], q0), a.tokens) - q0;
 }
 
-__device__ __forceinline__ int chunk_tiles(const ChunkArgs& a, int n) {
+__device__ __forceinline__ int chunk_tiles(ChunkArgsRef a, int n) {
   return (n * a.group + a.tile_rows - 1) / a.tile_rows;
 }
 
 // First key that the row at position p sees through the window (a row at a negative position sees nothing anyway).
 __device__ __forceinline__ int chunk_window_start(int p, int window) { return max(p, 0) - window + 1; }
 
-__device__ __forceinline__ ChunkTile chunk_geometry(const ChunkArgs& a, int b, int index) {
+__device__ __forceinline__ ChunkTile chunk_geometry(ChunkArgsRef a, int b, int index) {
   ChunkTile t;
   int n;
   t.b = b;
@@ -109,16 +121,54 @@ struct ChunkDims {
   static constexpr int kSlices = kFull + kTail;
   static constexpr int kBlocks = D / 16;       // chunks of the cache, blocks of 16 d of O^T
   static constexpr int kWaves = chunk_waves(D), kThreads = kWaves * kWave;
-  static constexpr int kTile = D <= 192 ? 64 : 32;        // tokens of a shared tile: what the registers leave room for
+  static constexpr int kTile = D <= 176 ? 64 : 32;        // tokens of a shared tile: what LDS has room for
   static constexpr int kStreamBlocks = 2;                 // column blocks of the stream path
-  static constexpr int kLds = 4 * kTile * D * 2;          // two buffers of K and V
+  static constexpr int kStages = 16 * kTile * D <= 128 * 1024 ? 4 : 3;  // tiles of K, and of V, in LDS
+  static constexpr int kPagesLds = kThreads * 4 * 4;      // page numbers of the tokens that a thread copies, four tiles
+  static constexpr int kLds = 2 * kStages * kTile * D * 2 + kPagesLds;
   static constexpr int kStreamLds = kWaves * 32 * D * 2;
   static constexpr int kJoinBlocks = 4;                   // blocks of O^T joined at a time: 64 KiB of LDS, or 32
   static constexpr int kJoinLds = kWaves * 16 * kStreamBlocks * kJoinBlocks * 16 * 4;
   static constexpr int kMain = kLds > kStreamLds ? (kLds > kJoinLds ? kLds : kJoinLds) : (kStreamLds > kJoinLds ? kStreamLds : kJoinLds);
   static constexpr int kSmall = 2 * kWaves * 32 * 4 + 16;         // joined maxima and sums, flags
   static constexpr int kPlan = (3 * kChunkMaxTiles + 1) * 4;
+  static_assert(kMain + kSmall + kPlan <= 160 * 1024, "LDS of a CU");
 };
+
+__device__ __forceinline__ uint32_t chunk_lds_address(const void* p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
+}
+
+// 16 bytes per lane from memory to LDS, lane l's to to + 16 l.  M0 carries the address; nothing else in these kernels uses it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void chunk_copy16(const f16* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0");
+}
+__device__ __forceinline__ void chunk_copy4(const int32_t* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "m0");
+}
+#pragma clang diagnostic pop
+
+// f(0), ..., f(N-1) with the numbers as types
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void chunk_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    chunk_for<N, I + 1>(f);
+  }
+}
+
+// All but the last N copies have arrived, and LDS reads and writes are done.
+template <int N>
+__device__ __forceinline__ void chunk_wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void chunk_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 typedef __fp16 ChunkTr __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) ChunkTr ChunkTrLds;
@@ -127,16 +177,26 @@ __device__ __forceinline__ f16x4 chunk_read_tr(const f16* lds) {
   return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((ChunkTrLds*)lds));
 }
 
-// Largest of the four lanes n, n + 16, n + 32, n + 48, in all four.  (The swaps exchange halves and quarters of the wave
-// between two registers; written as assembly because the compiler folds the builtins' two results into one when both
-// operands are the same value.  Their two wait states are part of it.)
-__device__ __forceinline__ float chunk_max4(float x) {
-  float y = x;
-  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-  x = fmaxf(x, y);
-  y = x;
-  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-  return fmaxf(x, y);
+// Maxima in assembly: fmaxf would first quiet each operand that comes from the matrix core or from assembly, an instruction
+// more for each of them.
+__device__ __forceinline__ float chunk_max3(float a, float b, float c) {
+  asm("v_max3_f32 %0, %0, %1, %2" : "+v"(a) : "v"(b), "v"(c));
+  return a;
+}
+__device__ __forceinline__ float chunk_max2(float a, float b) {
+  asm("v_max_f32 %0, %0, %1" : "+v"(a) : "v"(b));
+  return a;
+}
+// Largest of the four lanes n, n + 16, n + 32, n + 48, in all four, of two values.  (The swaps exchange halves and quarters of
+// the wave between two registers; in assembly because the compiler folds the builtins' two results into one when both operands
+// are the same value.  Their two wait states are part of it.)
+__device__ __forceinline__ void chunk_max4(float& a, float& b) {
+  float c = a, d = b;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\tv_permlane32_swap_b32 %2, %3" : "+v"(a), "+v"(c), "+v"(b), "+v"(d));
+  a = chunk_max2(a, c), b = chunk_max2(b, d);
+  c = a, d = b;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\tv_permlane16_swap_b32 %2, %3" : "+v"(a), "+v"(c), "+v"(b), "+v"(d));
+  a = chunk_max2(a, c), b = chunk_max2(b, d);
 }
 __device__ __forceinline__ float chunk_sum4(float x) {
   x += __shfl_xor(x, 16);
@@ -156,10 +216,15 @@ __device__ __forceinline__ bool chunk_not_finite(f16x8 v) {
 
 // Offset (in halfs) of token tok of the tile's sequence, from the start of the cache's kv head 0; entries outside the cache
 // read the nearest page.
-__device__ __forceinline__ int64_t chunk_token_offset(const ChunkArgs& a, const int32_t* table, int tok, int64_t page_elems) {
-  const int blk = (int)((uint64_t)(uint32_t)tok * a.block_magic >> a.block_shift);  // tok / block_size
-  const int page = min(max(table[blk], 0), a.num_blocks - 1);
-  return page * page_elems + (int64_t)(tok - blk * a.block_size) * 16;
+__device__ __forceinline__ int chunk_block(ChunkArgsRef a, int tok) {
+  return (int)((uint64_t)(uint32_t)tok * a.block_magic >> a.block_shift);  // tok / block_size
+}
+__device__ __forceinline__ int64_t chunk_page_offset(ChunkArgsRef a, int entry, int tok, int blk, int64_t page_elems) {
+  return min(max(entry, 0), a.num_blocks - 1) * page_elems + (int64_t)(tok - blk * a.block_size) * 16;
+}
+__device__ __forceinline__ int64_t chunk_token_offset(ChunkArgsRef a, const int32_t* table, int tok, int64_t page_elems) {
+  const int blk = chunk_block(a, tok);
+  return chunk_page_offset(a, table[blk], tok, blk, page_elems);
 }
 
 template <int D, int CB>
@@ -176,7 +241,7 @@ struct ChunkQuery {
 };
 
 template <int D, int CB>
-__device__ __forceinline__ void chunk_load_query(const ChunkArgs& a, const ChunkTile& t, int head, int first_row, int n, int kg,
+__device__ __forceinline__ void chunk_load_query(ChunkArgsRef a, const ChunkTile& t, int head, int first_row, int n, int kg,
                                                  ChunkQuery<D, CB>& q) {
   using Dims = ChunkDims<D>;
 #pragma unroll
@@ -209,34 +274,56 @@ __device__ __forceinline__ void chunk_init(ChunkState<D, CB>& st) {
 
 // Scores out of sight become -inf.  Lane (row n, kg) has tokens token0 + 16g + 4kg + i.
 template <int CB, int KG>
-__device__ __forceinline__ void chunk_mask(float (&s)[CB][KG][4], const int (&pos)[CB], int token0, int ctx, int window, int kg) {
+__device__ __forceinline__ void chunk_mask(f32x4 (&s)[CB][KG], const int (&pos)[CB], int token0, int ctx, int window, int kg) {
 #pragma unroll
   for (int c = 0; c < CB; ++c) {
-    const int last = min(pos[c], ctx - 1);
-    const int first = window > 0 ? pos[c] - window + 1 : 0;
+    const int last = min(pos[c], ctx - 1), first = window > 0 ? max(pos[c] - window + 1, 0) : 0;
+    const bool any = last >= first;
+    // tokens first .. last, in one unsigned comparison; where there are none, no token
+    const uint32_t span = any ? (uint32_t)(last - first) : 0u;
+    const uint32_t at = any ? (uint32_t)(token0 + 4 * kg - first) : 0x40000000u;
 #pragma unroll
     for (int g = 0; g < KG; ++g)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = token0 + 16 * g + 4 * kg + i;
-        if (tok > last || tok < first) s[c][g][i] = -__builtin_inff();
-      }
+      for (int i = 0; i < 4; ++i)
+        if (at + (16 * g + i) > span) s[c][g][i] = -__builtin_inff();
   }
 }
 
-// Online softmax; leaves the weights in s (fp32) and returns them packed as P^T operands of 32 tokens each.
+// Scores as the matrix core left them.  Its results may be read six wait states after it (four passes and two); the
+// compiler cannot tell for the assembly that reads them below, so the wait is part of handing them over.
+template <int CB, int KG>
+__device__ __forceinline__ void chunk_settle(f32x4 (&acc)[CB][KG]) {
+  static_assert(CB == 2 && (KG == 2 || KG == 4), "operands are listed");
+  if constexpr (KG == 4)
+    asm volatile("s_nop 7" : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[0][2]), "+v"(acc[0][3]), "+v"(acc[1][0]), "+v"(acc[1][1]), "+v"(acc[1][2]), "+v"(acc[1][3]));
+  else
+    asm volatile("s_nop 7" : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1]));
+}
+
+// Online softmax over settled scores; returns the weights packed as P^T operands of 32 tokens each.
 template <int D, int CB, int KG>
-__device__ __forceinline__ void chunk_softmax(float (&s)[CB][KG][4], ChunkState<D, CB>& st, f16x8 (&p)[CB][KG / 2]) {
+__device__ __forceinline__ void chunk_softmax(f32x4 (&s)[CB][KG], float scale, ChunkState<D, CB>& st, f16x8 (&p)[CB][KG / 2]) {
   float top[CB];
   bool moved = false;
 #pragma unroll
   for (int c = 0; c < CB; ++c) {
-    float m = s[c][0][0];
+    float m[2];  // two chains: a wave computes its softmax alone on its SIMD's vector unit
 #pragma unroll
-    for (int g = 0; g < KG; ++g)
+    for (int h = 0; h < 2; ++h) {
+      m[h] = chunk_max3(s[c][h][0], s[c][h][1], s[c][h][2]);
+      if constexpr (KG == 4) {
+        m[h] = chunk_max3(m[h], s[c][h][3], s[c][h + 2][0]);
+        m[h] = chunk_max3(m[h], s[c][h + 2][1], s[c][h + 2][2]);
+      }
+    }
+    m[0] = chunk_max3(m[0], s[c][KG - 2][3], s[c][KG - 1][3]);
+    top[c] = chunk_max2(m[0], m[1]);
+  }
+  chunk_max4(top[0], top[1]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m = fmaxf(m, s[c][g][i]);
-    top[c] = chunk_max4(m);
+  for (int c = 0; c < CB; ++c) {
+    top[c] *= scale;
     moved |= top[c] > st.ref[c] + kChunkSlack;
   }
   if (__builtin_amdgcn_ballot_w64(moved)) {
@@ -255,16 +342,16 @@ __device__ __forceinline__ void chunk_softmax(float (&s)[CB][KG][4], ChunkState<
 #pragma unroll
   for (int c = 0; c < CB; ++c) {
     const float base = kChunkLift - st.ref[c];
-    float sum = 0.f;
+    float sum[KG];
 #pragma unroll
-    for (int g = 0; g < KG; ++g)
+    for (int g = 0; g < KG; ++g) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float w = __builtin_amdgcn_exp2f(s[c][g][i] + base);
-        s[c][g][i] = w;
-        sum += w;
-      }
-    st.sum[c] += sum;
+      for (int i = 0; i < 4; ++i) s[c][g][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][g][i], scale, base));
+      sum[g] = (s[c][g][0] + s[c][g][1]) + (s[c][g][2] + s[c][g][3]);
+    }
+    float all = KG == 4 ? (sum[0] + sum[1]) + (sum[KG - 2] + sum[KG - 1]) : sum[0] + sum[1];
+    asm volatile("" : "+v"(all));  // added up here, not when the registers of all the weights have been held for long
+    st.sum[c] += all;
 #pragma unroll
     for (int h = 0; h < KG / 2; ++h)
 #pragma unroll
@@ -290,63 +377,24 @@ __device__ __forceinline__ void chunk_pv(const f16* v, int stride, int lane, con
     }
 }
 
-// The same for tiles whose V holds infinities or NaN that not every row may see: they are left out of the product, and what
-// a row does see of them is added as itself.  Which rows see any comes from products of indicators.
-template <int D, int CB, int KG>
-__device__ __forceinline__ void chunk_pv_guarded(const f16* v, int stride, int lane, const f16x8 (&p)[CB][KG / 2],
-                                                 const int (&pos)[CB], int token0, int ctx, int window,
-                                                 ChunkState<D, CB>& st) {
-  const int kg = lane >> 4;
-  // keeps the fragment reads, which are those of the ordinary product, from being moved in front of the branch, all at once
-  asm volatile("" : "+v"(lane));
-  const float inf = __builtin_inff();
-  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+// v with zeros in the place of infinities and NaN
+__device__ __forceinline__ f16x8 chunk_finite(f16x8 v) {
+  u32x4 u = __builtin_bit_cast(u32x4, v);
 #pragma unroll
-  for (int h = 0; h < KG / 2; ++h) {
-    f16x8 seen[CB];
-#pragma unroll
-    for (int c = 0; c < CB; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int tok = token0 + 32 * h + 16 * (e / 4) + 4 * kg + e % 4;
-        seen[c][e] = tok <= min(pos[c], ctx - 1) && (window <= 0 || tok > pos[c] - window) ? (f16)1.0f : (f16)0.0f;
-      }
-#pragma unroll
-    for (int db = 0; db < ChunkDims<D>::kBlocks; ++db) {
-      const f16* at = v + db * stride + 2 * h * 256 + lane * 4;
-      const f16x4 lo = chunk_read_tr(at), hi = chunk_read_tr(at + 256);
-      const f16x8 vt = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      f16x8 finite, up, down;  // NaN counts as both infinities
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = (float)vt[e];
-        finite[e] = __builtin_fabsf(x) < inf ? vt[e] : (f16)0.0f;
-        up[e] = x == inf || x != x ? (f16)1.0f : (f16)0.0f;
-        down[e] = x == -inf || x != x ? (f16)1.0f : (f16)0.0f;
-      }
-#pragma unroll
-      for (int c = 0; c < CB; ++c) {
-        const f32x4 ups = __builtin_amdgcn_mfma_f32_16x16x32_f16(up, seen[c], zero4, 0, 0, 0);
-        const f32x4 downs = __builtin_amdgcn_mfma_f32_16x16x32_f16(down, seen[c], zero4, 0, 0, 0);
-        st.o[c][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(finite, p[c][h], st.o[c][db], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (ups[i] > 0.f) st.o[c][db][i] += inf;
-          if (downs[i] > 0.f) st.o[c][db][i] -= inf;
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);  // one block at a time: a rare path must not cost the others their registers
-    }
+  for (int i = 0; i < 4; ++i) {
+    if ((u[i] & 0x7c00u) == 0x7c00u) u[i] &= 0xffff0000u;
+    if ((u[i] & 0x7c000000u) == 0x7c000000u) u[i] &= 0x0000ffffu;
   }
+  return __builtin_bit_cast(f16x8, u);
 }
 
 // Where a row's result goes: the outputs (part < 0) or slot `part` of the partial results.
 template <int D>
-__device__ __forceinline__ int64_t chunk_out_row(const ChunkArgs& a, const ChunkTile& t, int head, int r) {
+__device__ __forceinline__ int64_t chunk_out_row(ChunkArgsRef a, const ChunkTile& t, int head, int r) {
   const int row = t.row0 + r, token = row / a.group;
   return (int64_t)(t.q0 + token) * a.num_heads + head * a.group + (row - token * a.group);
 }
-__device__ __forceinline__ int64_t chunk_part_row(const ChunkArgs& a, int head, int part, int r) {
+__device__ __forceinline__ int64_t chunk_part_row(ChunkArgsRef a, int head, int part, int r) {
   return ((int64_t)head * 2 * a.shares + part) * a.part_rows + r;
 }
 // log-sum-exp (natural) of weights exp2(s - ref + kChunkLift) that add up to sum
@@ -354,9 +402,41 @@ __device__ __forceinline__ float chunk_lse(float ref, float sum) {
   return sum > 0.f || sum != sum ? (ref - kChunkLift + __builtin_amdgcn_logf(sum)) * kChunkLn2 : -__builtin_inff();
 }
 
+// Rows that see only a part of the `width` tokens from token0 on: those in front of the last of them, those whose window begins
+// behind the first; and tokens behind the context.
+__device__ __forceinline__ bool chunk_at_edge(ChunkArgsRef a, int token0, int width, int p_first, int p_last, int ctx) {
+  return token0 + width - 1 > p_first || token0 + width > ctx ||
+         (a.window > 0 && token0 < chunk_window_start(p_last, a.window));
+}
+
+// Adds to results that have been stored what their rows see of infinities and NaN in V at the edges, where these were left out
+// of the products.  Rare, and outside of the loops, whose registers it must not cost: a thread takes an element of the head.
+template <int D>
+__device__ void chunk_add_not_finite(ChunkArgsRef a, const ChunkTile& t, int head, int k0, int k1, int width, int part) {
+  __syncthreads();  // the results are stored
+  const int64_t page_elems = (int64_t)a.num_kv_heads * D * a.block_size;
+  const int32_t* table = a.block_tables + (int64_t)t.b * a.max_pages;
+  for (int d = threadIdx.x; d < D; d += ChunkDims<D>::kThreads)
+    for (int tok = k0; tok < k1; ++tok) {
+      if (!chunk_at_edge(a, k0 + (tok - k0) / width * width, width, t.p_first, t.p_last, t.ctx)) continue;
+      const f16 v = a.value_cache[chunk_token_offset(a, table, tok, page_elems) + ((int64_t)head * D + d / 16 * 16) * a.block_size + d % 16];
+      if ((__builtin_bit_cast(uint16_t, v) & 0x7c00u) != 0x7c00u) continue;
+      for (int r = 0; r < t.rows; ++r) {
+        const int p = t.p_first + (t.row0 + r) / a.group - t.row0 / a.group;
+        if (tok > p || (a.window > 0 && tok <= p - a.window)) continue;
+        if (part < 0) {
+          f16* o = a.out + chunk_out_row<D>(a, t, head, r) * D + d;
+          *o = (f16)((float)*o + (float)v);
+        } else {
+          a.part_o[chunk_part_row(a, head, part, r) * D + d] += (float)v;
+        }
+      }
+    }
+}
+
 // Keys k0 .. k1-1 (k0 a multiple of the tile) for a tile of many rows.
 template <int D>
-__device__ __forceinline__ void chunk_run_tile(const ChunkArgs& a, const ChunkTile& t, int head, int k0, int k1, int part,
+__device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& t, int head, int k0, int k1, int part,
                                                unsigned char* lds, int* flags) {
   using Dims = ChunkDims<D>;
   constexpr int KT = Dims::kTile, KG = KT / 16, CB = 2;
@@ -375,133 +455,223 @@ __device__ __forceinline__ void chunk_run_tile(const ChunkArgs& a, const ChunkTi
   const int wp_first = t.p_first + ((t.row0 + first_row) / a.group - t.row0 / a.group);
   const int wp_last = t.p_first + ((t.row0 + min(first_row + 31, t.rows - 1)) / a.group - t.row0 / a.group);
 
-  const int my_token = (threadIdx.x >> 1) & (KT - 1), my_chunk = threadIdx.x / kPieces;
+  // Copies: this thread's 16-byte pieces are piece threadIdx.x of every kStep chunks, all of one token.
+  const int my_token = (threadIdx.x >> 1) & (KT - 1), my_chunk = __builtin_amdgcn_readfirstlane(threadIdx.x / kPieces);
   const int64_t page_elems = (int64_t)a.num_kv_heads * D * a.block_size;
   const int64_t chunk_elems = (int64_t)a.block_size * 16;
   const int64_t lane_off = (int64_t)head * D * a.block_size + (threadIdx.x & 1) * 8 + my_chunk * chunk_elems;
   const int32_t* table = a.block_tables + (int64_t)t.b * a.max_pages;
-  f16x8 kreg[kRounds], vreg[kRounds];
-  auto offset_of = [&](int kt) { return chunk_token_offset(a, table, min(kt + my_token, t.ctx - 1), page_elems) + lane_off; };
-  auto load = [&](int64_t off) {
+  f16* const k_ring = reinterpret_cast<f16*>(lds);
+  f16* const v_ring = k_ring + Dims::kStages * KT * D;
+  const uint32_t lds_base = chunk_lds_address(lds);
+  const uint32_t k_to = lds_base + wave * (kWave * 16), v_to = k_to + Dims::kStages * KT * D * 2;  // this wave's pieces of a tile
+  auto token_of = [&](int tile) { return min(k0 + tile * KT + my_token, t.ctx - 1); };
+  // Page numbers come through LDS too (a wave's own, tile i in slot i % 4): waiting for an ordinary load would be waiting for all
+  // copies issued in front of it.
+  constexpr int kPagesAt = Dims::kLds - Dims::kPagesLds;
+  const int32_t* const my_pages = reinterpret_cast<const int32_t*>(lds + kPagesAt) + wave * (4 * kWave);
+  auto copy_page = [&](int tile) { chunk_copy4(table + chunk_block(a, token_of(tile)), lds_base + kPagesAt + wave * (4 * kWave * 4) + (tile & 3) * (kWave * 4)); };
+  auto offset_of = [&](int tile) {
+    const int tok = token_of(tile);
+    return chunk_page_offset(a, my_pages[(tile & 3) * kWave + lane], tok, chunk_block(a, tok), page_elems) + lane_off;
+  };
+  auto copy_round = [&](const f16* cache, int64_t off, uint32_t ring, int slot, int r) {
+    if ((Dims::kBlocks % kStep == 0) || my_chunk + r * kStep < Dims::kBlocks)
+      chunk_copy16(cache + off + r * kStep * chunk_elems, ring + slot * (KT * D * 2) + r * (Dims::kThreads * 16));
+  };
+  auto copy = [&](const f16* cache, int64_t off, uint32_t ring, int slot) {
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r)
-      if ((Dims::kBlocks % kStep == 0) || my_chunk + r * kStep < Dims::kBlocks) {
-        kreg[r] = ld128(a.key_cache + off + r * kStep * chunk_elems);
-        vreg[r] = ld128(a.value_cache + off + r * kStep * chunk_elems);
-      }
+    for (int r = 0; r < kRounds; ++r) copy_round(cache, off, ring, slot, r);
   };
-  // rows that see a tile only in part: behind the first row's position, or in front of the last row's window
-  auto at_edge = [&](int kt, int p_first, int p_last) {
-    return kt + KT - 1 > p_first || kt + KT > t.ctx || (a.window > 0 && kt < chunk_window_start(p_last, a.window));
-  };
-  f16* buffer = reinterpret_cast<f16*>(lds);
-  auto store = [&](int kt, int which) {
-    f16* k = buffer + which * 2 * KT * D + threadIdx.x * 8;
-    f16* v = k + KT * D;
-    const bool beyond = kt + my_token >= t.ctx;
+  // V rows behind the context become zeros, infinities and NaN at an edge too (and are noted): by the thread that copied them
+  auto patch = [&](int tile, int slot) {
+    const int kt = k0 + tile * KT;
+    if (!chunk_at_edge(a, kt, KT, t.p_first, t.p_last, t.ctx)) return;
     bool bad = false;
-    const f16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
     for (int r = 0; r < kRounds; ++r)
       if ((Dims::kBlocks % kStep == 0) || my_chunk + r * kStep < Dims::kBlocks) {
-        if (beyond) vreg[r] = zero8;
-        bad |= chunk_not_finite(vreg[r]);
-        st128(k + r * Dims::kThreads * 8, kreg[r]);
-        st128(v + r * Dims::kThreads * 8, vreg[r]);
+        f16* at = v_ring + slot * KT * D + (threadIdx.x + r * Dims::kThreads) * 8;
+        f16x8 x = ld128(at);
+        if (kt + my_token >= t.ctx) x = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        bad |= chunk_not_finite(x);
+        st128(at, chunk_finite(x));
       }
-    if (bad && at_edge(kt, t.p_first, t.p_last)) flags[which] = kt;
+    if (bad) flags[0] = 1;
   };
 
+  // The loop is cut into a phase for the matrix core (P V of the tile before, then the scores of this one) and one for the
+  // vector units (the softmax), with a barrier behind each, and waves 4-7, which share their SIMDs with waves 0-3, run one
+  // phase behind these: while one wave of a SIMD keeps the matrix core busy the other one computes weights.
+  //   phase 2j: waves 0-3 P V(j-1), S(j), waves 4-7 softmax(j-1);  phase 2j+1: waves 4-7 P V(j-1), S(j), waves 0-3 softmax(j)
+  // K and V go straight to LDS, in rings of n = kStages tiles each.  At the start of its phase for tile j a wave issues its copies
+  // for K(j+n-1) and V(j+n-2), into the slots of K(j-1) and V(j-2), which waves 4-7 read last, in phase 2j-1, and for the page
+  // numbers of tile j+2n-2.  At the end of that phase it waits for all but those of the last n-2 tiles: K(j+1) and V(j), first
+  // read in phase 2j+2, behind the barriers of both halves, and the page numbers of tile j+n, read at its next phase's start,
+  // have then arrived.
+  // The copies are assembly that the compiler does not count (it would turn every wait for an LDS read into a wait for all of
+  // them); a wave issues at least kCopies per tile.
+  constexpr int kAhead = Dims::kStages - 1, kCopies = 2 * (Dims::kBlocks / kStep) + 1;
+  const int tiles = k0 < k1 ? (k1 - k0 + KT - 1) / KT : 0;
+  const bool second = wave >= 4;
   __syncthreads();  // the last item's reads of LDS are done
-  if (threadIdx.x < 2) flags[threadIdx.x] = -1;
-  __syncthreads();
-  if (k0 < k1) {
-    load(offset_of(k0));
-    store(k0, 0);
+  if (threadIdx.x == 0) flags[0] = 0;
+  int64_t off_v = 0;  // of V(j+n-2)
+  for (int i = 0; i < min(tiles, kAhead); ++i) {
+    off_v = chunk_token_offset(a, table, token_of(i), page_elems) + lane_off;
+    copy(a.key_cache, off_v, k_to, i);
+    if (i + 1 < kAhead) copy(a.value_cache, off_v, v_to, i);
   }
-  int64_t next = k0 + KT < k1 ? offset_of(k0 + KT) : 0;
-  __syncthreads();
-  int which = 0;
-  for (int kt = k0; kt < k1; kt += KT, which ^= 1) {
-    const bool more = kt + KT < k1;
-    if (more) load(next);
-    if (kt + 2 * KT < k1) next = offset_of(kt + 2 * KT);
-    if (live && kt <= wp_last && (a.window <= 0 || kt + KT > chunk_window_start(wp_first, a.window))) {
-      const f16* k = buffer + which * 2 * KT * D;
-      const f16* v = k + KT * D;
-      f32x4 acc[CB][KG];
-      const f16* kfrag = k + (kg >> 1) * KT * 16 + n * 16 + (kg & 1) * 8;
-#pragma unroll
-      for (int g = 0; g < KG; ++g) {
-#pragma unroll
-        for (int c = 0; c < CB; ++c) acc[c][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < Dims::kSlices; ++s) {
-          f16x8 kf;
-          if (s < Dims::kFull) {
-            kf = ld128(kfrag + s * 2 * KT * 16 + g * 256);
-          } else {
-            kf = ld128(k + s * 2 * KT * 16 + g * 256 + n * 16 + (kg & 1) * 8);
-            if (kg >= 2) kf = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-          }
-#pragma unroll
-          for (int c = 0; c < CB; ++c)
-            acc[c][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q.d[c][s], acc[c][g], 0, 0, 0);
-        }
-      }
-      float s[CB][KG][4];
-#pragma unroll
-      for (int c = 0; c < CB; ++c)
-#pragma unroll
-        for (int g = 0; g < KG; ++g)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[c][g][i] = acc[c][g][i] * a.scale_log2;
-      const bool edge = at_edge(kt, wp_first, wp_last);
-      if (edge) chunk_mask<CB, KG>(s, q.pos, kt, t.ctx, a.window, kg);
-      f16x8 p[CB][KG / 2];
-      chunk_softmax<D, CB, KG>(s, st, p);
-      if (edge && flags[which] == kt)
-        chunk_pv_guarded<D, CB, KG>(v, KT * 16, lane, p, q.pos, kt, t.ctx, a.window, st);
-      else
-        chunk_pv<D, CB, KG>(v, KT * 16, lane, p, st);
-    }
-    if (more) store(kt + KT, which ^ 1);
-    __syncthreads();
-  }
+  for (int i = kAhead; i < min(tiles, 2 * kAhead); ++i) copy_page(i);
+  chunk_wait_copies<0>();
+  chunk_barrier();
 
-  if (!live) return;
+  f16x8 p[CB][KG / 2];
+  int j = 0, slot = 0, last_slot = Dims::kStages - 1;  // of K(j) and V(j), and of K(j-1) and V(j-1)
+  const f16* const k_lane = k_ring + (kg >> 1) * KT * 16 + n * 16 + (kg & 1) * 8;  // fragment s, group g: + s * 2 * KT * 16 + g * 256
+  const f16* const k_half = k_ring + Dims::kFull * 2 * KT * 16 + n * 16 + (kg & 1) * 8;
+  const f16* const v_lane = v_ring + lane * 4;
+  // steady: in the middle of an item, where every step issues all of its copies and no row's view ends
+  auto step = [&](auto pv, auto score, auto steady) {
+    constexpr bool kPv = decltype(pv)::value, kScore = decltype(score)::value, kSteady = decltype(steady)::value;
+    // slot j+n-1 = slot j-1; slot j+n-2 = slot j-2
+    const int v_slot = last_slot > 0 ? last_slot - 1 : kAhead;
+    if constexpr (!kSteady) {
+      if (j + kAhead - 1 < tiles) copy(a.value_cache, off_v, v_to, v_slot);
+      if (j + kAhead < tiles) {
+        off_v = offset_of(j + kAhead);
+        copy(a.key_cache, off_v, k_to, last_slot);
+        copy_page(j + 2 * kAhead);  // (behind the last tile: of the last token, and not used)
+      }
+    }
+    const int kt = k0 + j * KT;
+    f32x4 acc[CB][KG];
+    // Fragments of V (two reads each), then of K (one), each for CB products; a fragment is read kRing fragments before its
+    // products, and a steady step issues a copy behind every second one, where the matrix core is busy.  The order is the one
+    // written here: left to itself the compiler reads each fragment right in front of its products and waits for LDS, and
+    // copies in front of them all would leave the matrix core idle.
+    constexpr int kRing = 4, kV = kPv ? Dims::kBlocks * (KG / 2) : 0, kK = kScore ? Dims::kSlices * KG : 0;
+    f16x8 ring[kRing];
+    const int v_at = last_slot * KT * D, k_at = slot * KT * D;
+    auto read = [&](auto at) {
+      constexpr int I = decltype(at)::value;
+      if constexpr (I < kV) {
+        const f16* from = v_lane + v_at + (I % Dims::kBlocks) * KT * 16 + 2 * (I / Dims::kBlocks) * 256;
+        const f16x4 lo = chunk_read_tr(from), hi = chunk_read_tr(from + 256);
+        ring[I % kRing] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      } else if constexpr (I < kV + kK) {
+        constexpr int S = (I - kV) / KG, G = (I - kV) % KG;
+        ring[I % kRing] = ld128((S < Dims::kFull ? k_lane + S * 2 * KT * 16 : k_half) + k_at + G * 256);
+      }
+    };
+    auto products = [&](auto at) {
+      constexpr int I = decltype(at)::value;
+      if constexpr (I < kV) {
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+          st.o[c][I % Dims::kBlocks] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[I % kRing], p[c][I / Dims::kBlocks], st.o[c][I % Dims::kBlocks], 0, 0, 0);
+      } else {
+        constexpr int S = (I - kV) / KG, G = (I - kV) % KG;
+        f16x8 kf = ring[I % kRing];
+        if constexpr (S >= Dims::kFull)
+          if (kg >= 2) kf = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+          acc[c][G] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q.d[c][S], S > 0 ? acc[c][G] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+      }
+    };
+    auto copies = [&](auto at) {
+      constexpr int I = decltype(at)::value;
+      if constexpr (kSteady && I % 2 == 1) {
+        constexpr int R = I / 2;
+        if constexpr (R < kRounds) copy_round(a.value_cache, off_v, v_to, v_slot, R);
+        if constexpr (R == kRounds) off_v = offset_of(j + kAhead);
+        if constexpr (R > kRounds && R <= 2 * kRounds) copy_round(a.key_cache, off_v, k_to, last_slot, R - kRounds - 1);
+        if constexpr (R == 2 * kRounds + 1) copy_page(j + 2 * kAhead);
+      }
+    };
+    __builtin_amdgcn_s_setprio(1);
+    chunk_for<kRing>([&](auto i) { read(i); });
+    __builtin_amdgcn_sched_barrier(0);
+    chunk_for<kV + kK>([&](auto i) {
+      products(i);
+      copies(i);
+      read(std::integral_constant<int, decltype(i)::value + kRing>{});
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    if constexpr (kScore) chunk_settle<CB, KG>(acc);
+    __builtin_amdgcn_s_setprio(0);
+    if (kSteady || j + kAhead < tiles) {
+      chunk_wait_copies<(kAhead - 1) * kCopies>();
+    } else {
+      chunk_wait_copies<0>();
+    }
+    if (!kSteady && j < tiles) patch(j, slot);
+    if (second) chunk_barrier();
+    if constexpr (kScore) {
+      if (!kSteady && chunk_at_edge(a, kt, KT, wp_first, wp_last, t.ctx)) chunk_mask<CB, KG>(acc, q.pos, kt, t.ctx, a.window, kg);
+      chunk_softmax<D, CB, KG>(acc, a.scale_log2, st, p);
+    }
+    if (!second) chunk_barrier();
+    ++j;
+    last_slot = slot;
+    slot = slot < kAhead ? slot + 1 : 0;
+  };
+  // A wave computes where one of its rows sees a tile, and only helps with the copies in front of that and behind it: loops of
+  // their own, because accumulators changed under a condition inside a loop are copied in it.
+  const std::true_type yes;
+  const std::false_type no;
+  const int w_first = a.window > 0 ? max(chunk_window_start(wp_first, a.window) - k0, 0) / KT : 0;
+  const int w_end = live && wp_last >= k0 ? min(tiles, (wp_last - k0) / KT + 1) : 0;
+  while (j <= tiles && j < min(w_first, w_end)) step(no, no, no);
+  if (j < w_end) {
+    step(no, yes, no);
+    // steady: every row sees the whole tile, and there are copies to issue (and room for them among the products)
+    const int inner = a.window > 0 ? (max(chunk_window_start(t.p_last, a.window) - k0, 0) + KT - 1) / KT : 0;
+    const int outer = min(min(w_end, tiles - kAhead), max(min(t.p_first + 1, t.ctx) - k0, 0) / KT);
+    if constexpr (Dims::kBlocks * (KG / 2) + Dims::kSlices * KG >= 4 * kRounds + 4) {
+      while (j < min(w_end, inner)) step(yes, yes, no);
+      while (j < outer) step(yes, yes, yes);
+    }
+    while (j < w_end) step(yes, yes, no);
+    step(yes, no, no);
+  }
+  while (j <= tiles) step(no, no, no);
+  ChunkArgsRef e = chunk_reread(a);
+
 #pragma unroll
   for (int c = 0; c < CB; ++c) {
     const int r = first_row + 16 * c + n;
     const float sum = chunk_sum4(st.sum[c]);
     if (r >= t.rows) continue;
     if (part < 0) {
-      const int64_t row = chunk_out_row<D>(a, t, head, r);
+      const int64_t row = chunk_out_row<D>(e, t, head, r);
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
       for (int db = 0; db < Dims::kBlocks; ++db) {
         f16x4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = (f16)(st.o[c][db][i] * inv);
-        *reinterpret_cast<f16x4*>(a.out + row * D + 16 * db + 4 * kg) = v;
+        *reinterpret_cast<f16x4*>(e.out + row * D + 16 * db + 4 * kg) = v;
       }
-      if (a.lse && kg == 0) a.lse[row] = chunk_lse(st.ref[c], sum);
+      if (e.lse && kg == 0) e.lse[row] = chunk_lse(st.ref[c], sum);
     } else {
-      const int64_t row = chunk_part_row(a, head, part, r);
+      const int64_t row = chunk_part_row(e, head, part, r);
 #pragma unroll
       for (int db = 0; db < Dims::kBlocks; ++db)
-        *reinterpret_cast<f32x4*>(a.part_o + row * D + 16 * db + 4 * kg) = st.o[c][db];
+        *reinterpret_cast<f32x4*>(e.part_o + row * D + 16 * db + 4 * kg) = st.o[c][db];
       if (kg == 0) {
-        a.part_ml[2 * row] = st.ref[c];
-        a.part_ml[2 * row + 1] = sum;
+        e.part_ml[2 * row] = st.ref[c];
+        e.part_ml[2 * row + 1] = sum;
       }
     }
   }
+  if (flags[0]) chunk_add_not_finite<D>(e, t, head, k0, k1, KT, part);
 }
 
 // Keys k0 .. k1-1 (k0 a multiple of the unit) for a tile of at most 16 * kStreamBlocks rows.
 template <int D>
-__device__ __forceinline__ void chunk_run_stream(const ChunkArgs& a, const ChunkTile& t, int head, int k0, int k1, int part,
+__device__ __forceinline__ void chunk_run_stream(ChunkArgsRef a, const ChunkTile& t, int head, int k0, int k1, int part,
                                                  unsigned char* lds, float* small) {
   using Dims = ChunkDims<D>;
   constexpr int CB = Dims::kStreamBlocks, KG = 2, kStep = 32 * Dims::kWaves;
@@ -546,6 +716,7 @@ __device__ __forceinline__ void chunk_run_stream(const ChunkArgs& a, const Chunk
 #pragma unroll
     for (int db = 0; db < Dims::kBlocks; ++db) vreg[db] = ld128_stream(a.value_cache + voff + db * chunk_elems);
   };
+  bool not_finite = false;
   int token0 = k0 + 32 * wave;
   if (token0 < k1) {
     offsets(token0);
@@ -565,39 +736,30 @@ __device__ __forceinline__ void chunk_run_stream(const ChunkArgs& a, const Chunk
         for (int s = 0; s < Dims::kSlices; ++s)
           acc[c][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kreg[g][s], q.d[c][s], acc[c][g], 0, 0, 0);
       }
-    float s[CB][KG][4];
-#pragma unroll
-    for (int c = 0; c < CB; ++c)
-#pragma unroll
-      for (int g = 0; g < KG; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[c][g][i] = acc[c][g][i] * a.scale_log2;
+    chunk_settle<CB, KG>(acc);
     if (more) load_k();
-    const bool edge = token0 + 31 > t.p_first || token0 + 32 > t.ctx || (a.window > 0 && token0 < chunk_window_start(t.p_last, a.window));
-    bool guarded = false;
     const f16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (edge) {
-      chunk_mask<CB, KG>(s, q.pos, token0, t.ctx, a.window, kg);
+    if (chunk_at_edge(a, token0, 32, t.p_first, t.p_last, t.ctx)) {
+      chunk_mask<CB, KG>(acc, q.pos, token0, t.ctx, a.window, kg);
       bool bad = false;
 #pragma unroll
       for (int db = 0; db < Dims::kBlocks; ++db) {
         if (token0 + (lane >> 1) >= t.ctx) vreg[db] = zero8;
         bad |= chunk_not_finite(vreg[db]);
+        vreg[db] = chunk_finite(vreg[db]);
       }
-      guarded = __builtin_amdgcn_ballot_w64(bad) != 0;
+      not_finite |= bad;
     }
 #pragma unroll
     for (int db = 0; db < Dims::kBlocks; ++db) st128(mine + db * 512 + lane * 8, vreg[db]);
     if (more) load_v();
     f16x8 p[CB][KG / 2];
-    chunk_softmax<D, CB, KG>(s, st, p);
-    if (guarded)
-      chunk_pv_guarded<D, CB, KG>(mine, 512, lane, p, q.pos, token0, t.ctx, a.window, st);
-    else
-      chunk_pv<D, CB, KG>(mine, 512, lane, p, st);
+    chunk_softmax<D, CB, KG>(acc, a.scale_log2, st, p);
+    chunk_pv<D, CB, KG>(mine, 512, lane, p, st);
   }
 
   // Join the waves: common reference and total of every row, then the accumulators, kJoinBlocks blocks of 16 d at a time.
+  ChunkArgsRef e = chunk_reread(a);
   float* refs = small;                        // [wave][row]
   float* sums = small + Dims::kWaves * 32;
 #pragma unroll
@@ -608,7 +770,7 @@ __device__ __forceinline__ void chunk_run_stream(const ChunkArgs& a, const Chunk
       sums[wave * 32 + 16 * c + n] = sum;
     }
   }
-  __syncthreads();
+  const bool add_not_finite = __syncthreads_or(not_finite);
   float factor[CB];
 #pragma unroll
   for (int c = 0; c < CB; ++c) {
@@ -643,27 +805,28 @@ __device__ __forceinline__ void chunk_run_stream(const ChunkArgs& a, const Chunk
       for (int w = 0; w < Dims::kWaves; ++w) sum += sums[w * 32 + r] * __builtin_amdgcn_exp2f(refs[w * 32 + r] - ref);
       const int d = db0 * 16 + 4 * d4;
       if (part < 0) {
-        const int64_t row = chunk_out_row<D>(a, t, head, r);
+        const int64_t row = chunk_out_row<D>(e, t, head, r);
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
         f16x4 o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = (f16)(v[j] * inv);
-        *reinterpret_cast<f16x4*>(a.out + row * D + d) = o;
-        if (a.lse && d == 0) a.lse[row] = chunk_lse(ref, sum);
+        *reinterpret_cast<f16x4*>(e.out + row * D + d) = o;
+        if (e.lse && d == 0) e.lse[row] = chunk_lse(ref, sum);
       } else {
-        const int64_t row = chunk_part_row(a, head, part, r);
-        *reinterpret_cast<f32x4*>(a.part_o + row * D + d) = v;
+        const int64_t row = chunk_part_row(e, head, part, r);
+        *reinterpret_cast<f32x4*>(e.part_o + row * D + d) = v;
         if (d == 0) {
-          a.part_ml[2 * row] = ref;
-          a.part_ml[2 * row + 1] = sum;
+          e.part_ml[2 * row] = ref;
+          e.part_ml[2 * row + 1] = sum;
         }
       }
     }
   }
+  if (add_not_finite) chunk_add_not_finite<D>(e, t, head, k0, k1, 32, part);
 }
 
 template <int D>
-__device__ __forceinline__ void chunk_run(const ChunkArgs& a, const ChunkTile& t, int head, int unit, int units, int part,
+__device__ __forceinline__ void chunk_run(ChunkArgsRef a, const ChunkTile& t, int head, int unit, int units, int part,
                                           unsigned char* lds, float* small) {
   const int k0 = (t.unit0 + unit) * kChunkUnit, k1 = min(t.hi, (t.unit0 + unit + units) * kChunkUnit);
   if (t.rows <= 16 * ChunkDims<D>::kStreamBlocks) {
@@ -676,7 +839,7 @@ __device__ __forceinline__ void chunk_run(const ChunkArgs& a, const ChunkTile& t
 
 // Sequence and number of tile `tile` (the same in all lanes), counting the sequences' tiles one after the other; false
 // where there are fewer.
-__device__ __forceinline__ bool chunk_find(const ChunkArgs& a, int tile, int& b, int& index) {
+__device__ __forceinline__ bool chunk_find(ChunkArgsRef a, int tile, int& b, int& index) {
   const int lane = threadIdx.x & (kWave - 1);
   int running = 0;
   for (int64_t base = 0; base < a.seqs; base += kWave) {
@@ -706,7 +869,8 @@ __device__ __forceinline__ bool chunk_find(const ChunkArgs& a, int tile, int& b,
 // One workgroup per (tile, kv head), kv heads next to each other so that a kv head's tiles run on one XCD (or few) and share
 // its K and V in that L2.  The last tiles of the sequences, which see the most keys, come first.
 template <int D>
-__global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) void chunk_tiles_kernel(ChunkArgs a) {
+__global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) void chunk_tiles_kernel(ChunkArgs) {
+  ChunkArgsRef a = chunk_args();
   extern __shared__ __attribute__((aligned(16))) unsigned char chunk_lds[];
   const int head = blockIdx.x % a.num_kv_heads;
   int b, index;
@@ -719,7 +883,8 @@ __global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) v
 // inside one share is written directly; of the others every share leaves a partial result, in slot 2w of share w if the tile
 // began in front of the share and in slot 2w + 1 if it began in it, which chunk_merge joins in the order of the keys.
 template <int D>
-__global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) void chunk_shares_kernel(ChunkArgs a) {
+__global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) void chunk_shares_kernel(ChunkArgs) {
+  ChunkArgsRef a = chunk_args();
   using Dims = ChunkDims<D>;
   extern __shared__ __attribute__((aligned(16))) unsigned char chunk_lds[];
   float* small = reinterpret_cast<float*>(chunk_lds + Dims::kMain);
@@ -797,8 +962,9 @@ __global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) v
     const int upto = min(end, to);
     const bool whole = begin == from && upto == to;
     const int part = whole ? -1 : 2 * share_index + (begin == from ? 1 : 0);
-    const ChunkTile t = chunk_geometry(a, __builtin_amdgcn_readfirstlane(seq[tile]), __builtin_amdgcn_readfirstlane(number[tile]));
-    chunk_run<D>(a, t, head, begin - from, upto - begin, part, chunk_lds, small);
+    ChunkArgsRef e = chunk_reread(a);
+    const ChunkTile t = chunk_geometry(e, __builtin_amdgcn_readfirstlane(seq[tile]), __builtin_amdgcn_readfirstlane(number[tile]));
+    chunk_run<D>(e, t, head, begin - from, upto - begin, part, chunk_lds, small);
     begin = upto;
     ++tile;
   }

@@ -12,7 +12,8 @@ AOPS_CHUNK_DIMS(AOPS_CHUNK_EXTERN)
 
 // Partial results of one tile and 16 of its rows: 16 lanes per row, each with the elements 4l + 64j ..+3.  The partial
 // results of a tile are joined in the order of their keys, whatever order they were made in.
-__global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int head_dim) {
+__global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs, int head_dim) {
+  ChunkArgsRef a = chunk_args();
   const int tile = blockIdx.x, head = blockIdx.y;
   const int from = a.plan[tile], to = a.plan[tile + 1], total = a.plan[a.max_tiles];
   const int share = max((total + a.shares - 1) / a.shares, 1);
