@@ -55,7 +55,7 @@ struct ChunkArgs {
   f16* out;
   float* lse;            // may be null
   float *part_o, *part_ml;  // partial results: [kv head][2 * shares][part_rows][D] and [..][2]
-  int32_t* plan;         // units in front of each tile (max_tiles + 1), sequence and number of each tile
+  int32_t* plan;         // units in front of each tile (max_tiles + 1), sequence and number of each tile, tiles to join
   int32_t tokens, seqs, num_heads, num_kv_heads, group, block_size, max_pages, num_blocks, window;
   int32_t max_tiles, tile_rows, shares, part_rows;  // shares: of the balanced partition, per kv head; 0: one workgroup per tile
   uint32_t block_magic, block_shift;  // x / block_size = x * magic >> shift, x < 2^31
@@ -99,8 +99,10 @@ __device__ __forceinline__ ChunkTile chunk_geometry(ChunkArgsRef a, int b, int i
   int n;
   t.b = b;
   chunk_seq(a, b, t.q0, n);
-  t.row0 = index * a.tile_rows;
-  t.rows = min(n * a.group - t.row0, a.tile_rows);
+  // the sequence's rows in even tiles (whole waves of 32): a nearly empty last one would take as long as a full one
+  const int tiles = chunk_tiles(a, n), per = ((n * a.group + tiles - 1) / tiles + 31) & ~31;
+  t.row0 = index * per;
+  t.rows = min(n * a.group - t.row0, per);
   const int len = max(a.context_lens[b], 0);
   t.ctx = (int)min((int64_t)len, (int64_t)a.max_pages * a.block_size);
   t.p_first = len - n + t.row0 / a.group;
@@ -957,6 +959,9 @@ __global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) v
   int tile = 0;
   for (int step = kChunkMaxTiles; step > 0; step >>= 1)  // the last tile that begins at or in front of `begin`
     if (tile + step < a.max_tiles && before[tile + step] <= begin) tile += step;
+  // for the join: the tile that this share continues, if it is the first one to do so
+  if (head == 0 && threadIdx.x == 0)
+    a.plan[3 * a.max_tiles + 1 + share_index] = begin < end && begin > before[tile] && before[tile] / share + 1 == share_index ? tile : -1;
   while (begin < end) {
     const int from = __builtin_amdgcn_readfirstlane(before[tile]), to = __builtin_amdgcn_readfirstlane(before[tile + 1]);
     const int upto = min(end, to);

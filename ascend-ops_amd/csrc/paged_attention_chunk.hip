@@ -10,39 +10,56 @@ namespace aops {
 
 AOPS_CHUNK_DIMS(AOPS_CHUNK_EXTERN)
 
-// Partial results of one tile and 16 of its rows: 16 lanes per row, each with the elements 4l + 64j ..+3.  The partial
-// results of a tile are joined in the order of their keys, whatever order they were made in.
-__global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs, int head_dim) {
+// Joins the partial results of a tile, in the order of their keys, whatever order they were made in: a wave per row.  The wave
+// first finds the row's common reference and total, a lane per partial result; then `lanes` lanes (a power of two from a
+// quarter of head_dim on) take four elements each, and the 64 / lanes groups of them every so many-th partial result, so that
+// the many partial results of a few rows are read side by side (one after the other they took 36 us of 127 for 32 rows of
+// 32 partial results).
+constexpr int kMergeWaves = 8;
+__global__ __launch_bounds__(kMergeWaves* kWave) void chunk_merge_kernel(ChunkArgs, int head_dim, int lanes, int rows_per_wave) {
   ChunkArgsRef a = chunk_args();
-  const int tile = blockIdx.x, head = blockIdx.y;
+  const int tile = a.plan[3 * a.max_tiles + 1 + blockIdx.z], head = blockIdx.x;
+  if (tile < 0) return;
   const int from = a.plan[tile], to = a.plan[tile + 1], total = a.plan[a.max_tiles];
   const int share = max((total + a.shares - 1) / a.shares, 1);
-  if (from >= to || from / share == (to - 1) / share) return;  // none, or written directly
   const ChunkTile t = chunk_geometry(a, a.plan[a.max_tiles + 1 + tile], a.plan[2 * a.max_tiles + 1 + tile]);
-  const int r = blockIdx.z * 16 + threadIdx.x / 16, l = threadIdx.x & 15;
-  if (r >= t.rows) return;
-  const int s0 = from / share, s1 = (to - 1) / share;
-  auto slot = [&](int s) { return chunk_part_row(a, head, 2 * s + (s == s0 ? 1 : 0), r); };
-  // (the first share's part begins in that share, all others' in front of theirs)
-  float ref = kChunkNegBig;
-  for (int s = s0; s <= s1; ++s) ref = fmaxf(ref, a.part_ml[2 * slot(s)]);
-  float sum = 0.f;
-  for (int s = s0; s <= s1; ++s)
-    sum += a.part_ml[2 * slot(s) + 1] * __builtin_amdgcn_exp2f(a.part_ml[2 * slot(s)] - ref);
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  const int64_t row = chunk_out_row<0>(a, t, head, r);
-  for (int d = 4 * l; d < head_dim; d += 64) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = s0; s <= s1; ++s) {
-      const int64_t at = slot(s);
-      v += *reinterpret_cast<const f32x4*>(a.part_o + at * head_dim + d) * __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int s0 = from / share, parts = (to - 1) / share - s0 + 1;
+  const int first = (blockIdx.y * kMergeWaves + threadIdx.x / kWave) * rows_per_wave;
+  for (int r = first; r < min(first + rows_per_wave, t.rows); ++r) {
+    // the first share's part begins in that share, all others' in front of theirs
+    auto slot = [&](int i) { return chunk_part_row(a, head, 2 * (s0 + i) + (i == 0 ? 1 : 0), r); };
+    float ref = kChunkNegBig;
+    for (int i = lane; i < parts; i += kWave) ref = fmaxf(ref, a.part_ml[2 * slot(i)]);
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) ref = fmaxf(ref, __shfl_xor(ref, m));
+    float sum = 0.f;
+    for (int i = lane; i < parts; i += kWave) {
+      const int64_t at = slot(i);
+      sum += a.part_ml[2 * at + 1] * __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
     }
+    sum = wave_sum(sum);
+    const int l = lane & (lanes - 1), groups = kWave / lanes;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (4 * l < head_dim) {
+#pragma unroll 4
+      for (int i = lane / lanes; i < parts; i += groups) {
+        const int64_t at = slot(i);
+        v += *reinterpret_cast<const f32x4*>(a.part_o + at * head_dim + 4 * l) * __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
+      }
+    }
+    for (int m = lanes; m < kWave; m <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], m);
+    if (lane >= lanes || 4 * l >= head_dim) continue;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const int64_t row = chunk_out_row<0>(a, t, head, r);
     f16x4 o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = (f16)(v[j] * inv);
-    *reinterpret_cast<f16x4*>(a.out + row * head_dim + d) = o;
+    *reinterpret_cast<f16x4*>(a.out + row * head_dim + 4 * l) = o;
+    if (a.lse && l == 0) a.lse[row] = chunk_lse(ref, sum);
   }
-  if (a.lse && l == 0) a.lse[row] = chunk_lse(ref, sum);
 }
 
 struct ChunkPlan {
@@ -58,18 +75,21 @@ static bool chunk_sizes_ok(int64_t tokens, int64_t seqs, int64_t num_heads, int6
          tokens <= 0x3fffffff / (num_heads / num_kv_heads) && max_pages <= 0x7ffffe00 / block_size;
 }
 
-// The balanced partition pays where whole tiles would leave CUs idle: fewer than four tiles per CU, and sequences long
-// enough (by what a row of the block table can hold) that a share is worth a partial result.
+// The balanced partition pays where whole tiles would leave CUs idle: fewer than two per CU, and sequences long enough (by what a
+// row of the block table can hold) that a share is worth a partial result; and where single sequences may be so long that one
+// of their tiles would outlast all others.  (24 sequences with a window of 1024, 16 kv heads, up to 544 tiles: 74 us in whole
+// tiles, 92 balanced; 5 prompts of 77 to 2000 tokens, 656 tiles: 92 and 124; 4096 tokens over 32768 keys, 520 tiles: 1750 and
+// 1775; 16 tokens over 131079 keys, 72 tiles of which 8 exist: 114 balanced, 2.7 ms in whole tiles.)
 static ChunkPlan chunk_plan(int64_t tokens, int64_t seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                             int64_t block_size, int64_t max_pages) {
   const int64_t group = num_heads / num_kv_heads, cus = device_cu_count(), tile_rows = chunk_rows((int)head_dim);
   ChunkPlan p = {(tokens * group + tile_rows - 1) / tile_rows + std::min(seqs, tokens), 0, 0, 16};
-  if (p.max_tiles <= kChunkMaxTiles && p.max_tiles * num_kv_heads < 4 * cus && num_kv_heads <= cus &&
-      max_pages * block_size > 4 * kChunkUnit) {
+  if (p.max_tiles <= kChunkMaxTiles && num_kv_heads <= cus &&
+      (p.max_tiles * num_kv_heads < 2 * cus ? max_pages * block_size > 4 * kChunkUnit : max_pages * block_size > 32 * kChunkUnit)) {
     p.shares = cus / num_kv_heads;
     p.part_rows = std::min<int64_t>(tile_rows, (tokens * group + 15) / 16 * 16);
     const size_t rows = (size_t)(num_kv_heads * 2 * p.shares * p.part_rows);
-    p.bytes = rows * (size_t)(head_dim + 2) * sizeof(float) + (size_t)(3 * p.max_tiles + 1) * sizeof(int32_t);
+    p.bytes = rows * (size_t)(head_dim + 2) * sizeof(float) + (size_t)(3 * p.max_tiles + 1 + p.shares) * sizeof(int32_t);
   }
   return p;
 }
@@ -147,7 +167,11 @@ extern "C" int aops_paged_attention_chunk_f16(const void* q, const void* key_cac
 #undef AOPS_CHUNK_CASE
   }
   if (e != hipSuccess || p.shares == 0) return record_launch_status(e);
-  chunk_merge_kernel<<<dim3((unsigned)p.max_tiles, (unsigned)num_kv_heads, (unsigned)((p.part_rows + 15) / 16)), 256, 0, st>>>(
-      a, (int)head_dim);
+  int lanes = 4;
+  while (4 * lanes < head_dim) lanes *= 2;
+  const int rows_per_wave = p.part_rows <= 64 ? 1 : 4, rows = kMergeWaves * rows_per_wave;
+  // (kv heads vary fastest, so that the few tiles of a small call are joined on all XCDs)
+  chunk_merge_kernel<<<dim3((unsigned)num_kv_heads, (unsigned)((p.part_rows + rows - 1) / rows), (unsigned)p.shares),
+                       kMergeWaves * kWave, 0, st>>>(a, (int)head_dim, lanes, rows_per_wave);
   return record_launch_status(hipGetLastError());
 }
