@@ -63,12 +63,12 @@ struct PlanOut {
   int32_t* place;
 };
 
-constexpr int kPlanWaves = 16;
-constexpr int kPlanPer = 8;  // counts per lane and tile
-constexpr int kPlanTile = kPlanWaves * kWave * kPlanPer;
+constexpr int kPlanWaves = 16;  // of a planning workgroup
+constexpr int kRowWaves = 4;    // of the others
 
-// Exclusive sum over the waves of a workgroup and the total; `sums`: kPlanWaves ints of LDS.
-__device__ __forceinline__ int plan_waves_before(int mine, int* sums, int& total) {
+// Exclusive sum over the waves of a workgroup and the total; `sums`: WAVES ints of LDS.
+template <int WAVES>
+__device__ __forceinline__ int waves_before(int mine, int* sums, int& total) {
   const int wave = threadIdx.x / kWave;
   __syncthreads();  // the last round's values have been read
   if ((threadIdx.x & (kWave - 1)) == 0) sums[wave] = mine;
@@ -76,7 +76,7 @@ __device__ __forceinline__ int plan_waves_before(int mine, int* sums, int& total
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kPlanWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     const int n = sums[w];
     before += w < wave ? n : 0;
     total += n;
@@ -84,28 +84,39 @@ __device__ __forceinline__ int plan_waves_before(int mine, int* sums, int& total
   return before;
 }
 
+// Sum over a workgroup.
+template <int WAVES>
+__device__ __forceinline__ int workgroup_sum(int mine, int* sums) {
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) mine += __shfl_xor(mine, d);
+  int total;
+  waves_before<WAVES>(mine, sums, total);
+  return total;
+}
+
 // One pass over the counts in page order: visit(page, count, is_free, free pages in front of it).  Returns the free pages.
-template <typename F>
-__device__ __forceinline__ int plan_scan(const int32_t* __restrict__ counts, int num_blocks, int* sums, F visit) {
+template <int WAVES, typename F>
+__device__ __forceinline__ int scan_counts(const int32_t* __restrict__ counts, int num_blocks, int* sums, F visit) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const uint64_t below = lane == 0 ? 0 : ~uint64_t(0) >> (kWave - lane);
+  constexpr int kPer = 8;  // counts per lane and tile
   int running = 0;
-  for (int64_t tile = 0; tile < num_blocks; tile += kPlanTile) {
-    const int64_t first = tile + wave * (kWave * kPlanPer) + lane;
-    int32_t c[kPlanPer];
-    uint64_t free[kPlanPer];
+  for (int64_t tile = 0; tile < num_blocks; tile += WAVES * kWave * kPer) {
+    const int64_t first = tile + wave * (kWave * kPer) + lane;
+    int32_t c[kPer];
+    uint64_t free[kPer];
     int mine = 0;
 #pragma unroll
-    for (int j = 0; j < kPlanPer; ++j) c[j] = first + j * kWave < num_blocks ? counts[first + j * kWave] : 1;
+    for (int j = 0; j < kPer; ++j) c[j] = first + j * kWave < num_blocks ? counts[first + j * kWave] : 1;
 #pragma unroll
-    for (int j = 0; j < kPlanPer; ++j) {
+    for (int j = 0; j < kPer; ++j) {
       free[j] = __builtin_amdgcn_ballot_w64(c[j] <= 0);
       mine += __builtin_popcountll(free[j]);
     }
     int total;
-    int rank = running + plan_waves_before(mine, sums, total);
+    int rank = running + waves_before<WAVES>(mine, sums, total);
 #pragma unroll
-    for (int j = 0; j < kPlanPer; ++j) {
+    for (int j = 0; j < kPer; ++j) {
       if (first + j * kWave < num_blocks)
         visit((int)(first + j * kWave), c[j], c[j] <= 0, rank + __builtin_popcountll(free[j] & below));
       rank += __builtin_popcountll(free[j]);
@@ -179,7 +190,7 @@ __global__ __launch_bounds__(kPlanWaves* kWave) void pages_plan_kernel(Tables t,
     if (i < requests) out.before[i] = (int)min((int64_t)asked + before + (upto - need), (int64_t)cap);
     asked = (int)min((int64_t)asked + total, (int64_t)cap);
   }
-  const int free = plan_scan(counts, num_blocks, sums, [&](int page, int32_t c, bool is_free, int rank) {
+  const int free = scan_counts<kPlanWaves>(counts, num_blocks, sums, [&](int page, int32_t c, bool is_free, int rank) {
     new_counts[page] = max(c, 0);
     if (is_free && rank < asked) out.list[rank] = page;
   });
@@ -187,6 +198,26 @@ __global__ __launch_bounds__(kPlanWaves* kWave) void pages_plan_kernel(Tables t,
 }
 
 // ------------------------------------------------------------------------------------------- fork
+// Copies the first `part` tokens of page src to page dst: workgroup y - 1 = cache * slices + slice, its slice of them.
+__device__ __forceinline__ void copy_last_page(const Tables& t, int32_t src, int32_t dst, int part, const Caches& caches,
+                                               uint32_t slices, int32_t num_blocks, uint32_t granules) {
+  if (src < 0 || src >= num_blocks) return;
+  const int64_t page_elems = (int64_t)granules * t.block_size * 16;
+  const uint32_t per_granule = 2u * part;  // 16-byte pieces of the used tokens; a page has `granules` such runs
+  const uint32_t pieces = granules * per_granule;
+  const uint32_t cache = (blockIdx.y - 1) / slices, slice = (blockIdx.y - 1) - cache * slices;
+  f16* base = caches.at[cache];
+  const uint32_t begin = (uint32_t)((uint64_t)pieces * slice / slices);
+  const uint32_t end = (uint32_t)((uint64_t)pieces * (slice + 1) / slices);
+  // i / per_granule by its reciprocal, rounded down: at most one too small
+  const uint32_t inverse = 0xffffffffu / per_granule;
+  copy_pieces(base + src * page_elems, base + dst * page_elems, begin, end, [&](uint32_t i) {
+    uint32_t c = __umulhi(i, inverse), rest = i - c * per_granule;
+    if (rest >= per_granule) ++c, rest -= per_granule;
+    return ((int64_t)c * t.block_size * 2 + rest) * 8;
+  });
+}
+
 // Workgroup (child, y): y == 0 writes the child's row; y - 1 = cache * slices + slice copies a slice of the used tokens
 // of the parent's last page.
 __global__ __launch_bounds__(256) void fork_kernel(Tables t, const int32_t* __restrict__ parents, Caches caches,
@@ -213,20 +244,7 @@ __global__ __launch_bounds__(256) void fork_kernel(Tables t, const int32_t* __re
     return;
   }
   if (!ok || part == 0) return;
-  const int32_t src = row[full];
-  if (src < 0 || src >= num_blocks) return;
-  const int64_t page_elems = (int64_t)granules * t.block_size * 16;
-  const int64_t from = src * page_elems, to = plan.list[rank] * page_elems;
-  const uint32_t per_granule = 2u * part;  // 16-byte pieces of the used tokens; a page has `granules` such runs
-  const uint32_t pieces = granules * per_granule;
-  const uint32_t cache = (blockIdx.y - 1) / slices, slice = (blockIdx.y - 1) - cache * slices;
-  f16* base = caches.at[cache];
-  const uint32_t begin = (uint32_t)((uint64_t)pieces * slice / slices);
-  const uint32_t end = (uint32_t)((uint64_t)pieces * (slice + 1) / slices);
-  copy_pieces(base + from, base + to, begin, end, [&](uint32_t i) {
-    const uint32_t c = i / per_granule;
-    return ((int64_t)c * t.block_size * 2 + (i - c * per_granule)) * 8;
-  });
+  copy_last_page(t, row[full], plan.list[rank], part, caches, slices, num_blocks, granules);
 }
 
 // ------------------------------------------------------------------------------------------- extend
@@ -279,11 +297,11 @@ __global__ __launch_bounds__(kPlanWaves* kWave) void compact_plan_kernel(const i
                                                                          int32_t num_blocks, int32_t* __restrict__ used_out,
                                                                          PlanOut out) {
   __shared__ int sums[kPlanWaves];
-  const int free = plan_scan(counts, num_blocks, sums, [](int, int32_t, bool, int) {});
+  const int free = scan_counts<kPlanWaves>(counts, num_blocks, sums, [](int, int32_t, bool, int) {});
   const int used = num_blocks - free;
   __shared__ int free_below;  // free pages in front of page `used`: the holes
   if (threadIdx.x == 0) free_below = used == num_blocks ? free : -1;
-  plan_scan(counts, num_blocks, sums, [&](int page, int32_t, bool is_free, int rank) {
+  scan_counts<kPlanWaves>(counts, num_blocks, sums, [&](int page, int32_t, bool is_free, int rank) {
     if (page == used) free_below = rank;
     if (is_free && page < used) out.list[rank] = page;
     // used pages in front of this one: page - rank; the ones behind `used` come after used - free_below others
@@ -301,6 +319,23 @@ __global__ __launch_bounds__(kPlanWaves* kWave) void compact_plan_kernel(const i
     out.head[0] = used;
     out.head[1] = holes;
     used_out[0] = used;
+  }
+}
+
+// Workgroup `wg` of `wgs` copies its share of the pages that move, a piece of one page in one cache at a time.
+template <typename FROM, typename TO>
+__device__ __forceinline__ void copy_moves(uint32_t wg, uint32_t wgs, int moves, const Caches& caches, int num_caches,
+                                           uint32_t chunks, int64_t page_elems, FROM from, TO to) {
+  const uint64_t per_move = (uint64_t)num_caches * chunks;
+  const uint64_t items = per_move * moves;
+  for (uint64_t i = wg; i < items; i += wgs) {
+    const uint32_t move = (uint32_t)(i / per_move), rest = (uint32_t)(i - move * per_move);
+    const uint32_t cache = rest / chunks, chunk = rest - cache * chunks;
+    const uint32_t begin = chunk * kCopyPieces;
+    const uint32_t end = (uint32_t)min((int64_t)begin + kCopyPieces, page_elems / 8);
+    f16* base = caches.at[cache];
+    copy_pieces(base + from(move) * page_elems, base + to(move) * page_elems, begin, end,
+                [](uint32_t j) { return (int64_t)j * 8; });
   }
 }
 
@@ -331,17 +366,228 @@ __global__ __launch_bounds__(256) void compact_kernel(Tables t, const int32_t* _
     }
     return;
   }
-  const uint64_t per_move = (uint64_t)num_caches * chunks;
-  const uint64_t items = per_move * moves;
-  for (uint64_t i = blockIdx.x - row_wgs; i < items; i += gridDim.x - row_wgs) {
-    const uint32_t move = (uint32_t)(i / per_move), rest = (uint32_t)(i - move * per_move);
-    const uint32_t cache = rest / chunks, chunk = rest - cache * chunks;
-    const uint32_t begin = chunk * kCopyPieces;
-    const uint32_t end = (uint32_t)min((int64_t)begin + kCopyPieces, page_elems / 8);
-    f16* base = caches.at[cache];
-    copy_pieces(base + plan.movers[move] * page_elems, base + plan.list[move] * page_elems, begin, end,
-                [](uint32_t j) { return (int64_t)j * 8; });
+  copy_moves(blockIdx.x - row_wgs, gridDim.x - row_wgs, moves, caches, num_caches, chunks, page_elems,
+             [&](int k) { return (int64_t)plan.movers[k]; }, [&](int k) { return (int64_t)plan.list[k]; });
+}
+
+// ------------------------------------------------------------------------------------------- small pools
+// The same operators in one launch, for pools of up to kSmallPool pages and tables of up to kSmallEntries entries: a decode
+// step's calls, where each launch counts (about 2 us on the host and as much between two kernels).  Every workgroup finds what it
+// needs of the plan itself, from counts that are a few KiB in the L2, and one workgroup makes the new counts, in LDS.
+constexpr int kSmallPool = 4096;
+constexpr int64_t kSmallEntries = 16384;
+
+// Pages asked for by the requests in front of request i; called by a workgroup of kRowWaves waves.
+template <bool FORK>
+__device__ __forceinline__ int asked_before(const Tables& t, const int32_t* who, int i, int* sums) {
+  int64_t mine = 0;
+  for (int k = threadIdx.x; k < i; k += kRowWaves * kWave) mine += plan_request<FORK>(t, who, k);
+  return workgroup_sum<kRowWaves>((int)min(mine, (int64_t)kSmallPool + 1), sums);
+}
+
+// Pages given out: the largest sum of leading requests that the free pages suffice for.
+template <bool FORK>
+__device__ __forceinline__ int given_out(const Tables& t, const int32_t* who, int requests, int free, int* sums) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int asked = 0, given = 0;
+  for (int64_t tile = 0; tile < requests; tile += kRowWaves * kWave) {
+    const int64_t i = tile + threadIdx.x;
+    int upto = i < requests ? min(plan_request<FORK>(t, who, (int)i), kSmallPool + 1) : 0;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
+    }
+    int total;
+    const int mine = __shfl(upto, kWave - 1);
+    upto += waves_before<kRowWaves>(mine, sums, total) + asked;
+    int fits = i < requests && upto <= free ? upto : 0;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) fits = max(fits, __shfl_xor(fits, d));
+    __syncthreads();
+    if (lane == 0) sums[threadIdx.x / kWave] = fits;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) given = max(given, sums[w]);
+    asked = min(asked + total, kSmallPool + 1);
   }
+  return given;
+}
+
+// Workgroup (child, y) as in fork_kernel; workgroup (children, 0) makes the counts and lengths.
+__global__ __launch_bounds__(kRowWaves* kWave) void fork_small_kernel(Tables t, const int32_t* __restrict__ parents,
+                                                                       int32_t children, Caches caches, uint32_t slices,
+                                                                       const int32_t* __restrict__ counts, int32_t num_blocks,
+                                                                       uint32_t granules, int32_t* __restrict__ child_tables,
+                                                                       int32_t* __restrict__ child_lens,
+                                                                       int32_t* __restrict__ new_counts) {
+  __shared__ int sums[kRowWaves];
+  __shared__ int fresh;
+  __shared__ int held[kSmallPool];
+  const int child = blockIdx.x;
+  if (child == children) {
+    if (blockIdx.y > 0) return;
+    const int free = scan_counts<kRowWaves>(counts, num_blocks, sums, [&](int page, int32_t c, bool, int) { held[page] = max(c, 0); });
+    const int given = given_out<true>(t, parents, children, free, sums);
+    scan_counts<kRowWaves>(counts, num_blocks, sums, [&](int page, int32_t, bool is_free, int rank) {
+      if (is_free && rank < given) atomicAdd(held + page, 1);
+    });
+    // shared pages, of the children whose own page (if they need one) is among those given out
+    int asked = 0;
+    const int lane = threadIdx.x & (kWave - 1);
+    for (int64_t tile = 0; tile < children; tile += kRowWaves * kWave) {
+      const int64_t i = tile + threadIdx.x;
+      const int need = i < children ? plan_request<true>(t, parents, (int)i) : 0;
+      int upto = need;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+      int total;
+      const int mine = __shfl(upto, kWave - 1);
+      upto += waves_before<kRowWaves>(mine, sums, total) + asked;
+      asked += total;
+      if (i < children) {
+        const int tokens = seq_tokens(t, parents[i]);
+        const bool ok = need == 0 || upto <= free;
+        child_lens[i] = ok ? tokens : 0;
+        if (ok)
+          for (int j = 0; j < tokens / t.block_size; ++j) {
+            const int32_t page = t.tables[(int64_t)parents[i] * t.width + j];
+            if (page >= 0 && page < num_blocks) atomicAdd(held + page, 1);
+          }
+      }
+    }
+    __syncthreads();
+    for (int p = threadIdx.x; p < num_blocks; p += kRowWaves * kWave) new_counts[p] = held[p];
+    return;
+  }
+  const int parent = parents[child];
+  const int tokens = seq_tokens(t, parent);
+  const int full = tokens / t.block_size, part = tokens - full * t.block_size;
+  const int32_t* row = t.tables + (int64_t)(tokens > 0 ? parent : 0) * t.width;
+  bool ok = true;
+  if (part > 0) {
+    const int rank = asked_before<true>(t, parents, child, sums);
+    const int free = scan_counts<kRowWaves>(counts, num_blocks, sums, [&](int page, int32_t, bool is_free, int r) {
+      if (is_free && r == rank) fresh = page;
+    });
+    ok = rank < free;
+    __syncthreads();
+  }
+  if (blockIdx.y == 0) {
+    int32_t* out = child_tables + (int64_t)child * t.width;
+    for (int j = threadIdx.x; j < t.width; j += 256) out[j] = !ok ? -1 : j < full ? row[j] : j == full && part > 0 ? fresh : -1;
+    return;
+  }
+  if (!ok || part == 0) return;
+  copy_last_page(t, row[full], fresh, part, caches, slices, num_blocks, granules);
+}
+
+// Workgroup `seq` writes the row of a sequence, workgroup `seqs` the counts.
+__global__ __launch_bounds__(kRowWaves* kWave) void extend_small_kernel(Tables t, const int32_t* __restrict__ wanted,
+                                                                         const int32_t* __restrict__ counts, int32_t num_blocks,
+                                                                         int32_t* __restrict__ new_tables,
+                                                                         int32_t* __restrict__ granted,
+                                                                         int32_t* __restrict__ new_counts) {
+  __shared__ int sums[kRowWaves];
+  const int seq = blockIdx.x;
+  if (seq == t.seqs) {
+    const int free = scan_counts<kRowWaves>(counts, num_blocks, sums, [](int, int32_t, bool, int) {});
+    const int given = given_out<false>(t, wanted, t.seqs, free, sums);
+    scan_counts<kRowWaves>(counts, num_blocks, sums, [&](int page, int32_t c, bool is_free, int rank) {
+      new_counts[page] = is_free ? (rank < given ? 1 : 0) : c;
+    });
+    return;
+  }
+  const int have_tokens = seq_tokens(t, seq), want = wanted[seq];
+  const int have = pages_of(have_tokens, t.block_size);
+  const int need = plan_request<false>(t, wanted, seq);
+  const int32_t* row = t.tables + (int64_t)seq * t.width;
+  int32_t* out = new_tables + (int64_t)seq * t.width;
+  bool ok = want > have_tokens && (int64_t)want <= (int64_t)t.width * t.block_size;
+  if (ok && need > 0) {
+    const int before = asked_before<false>(t, wanted, seq, sums);
+    const int free = scan_counts<kRowWaves>(counts, num_blocks, sums, [](int, int32_t, bool, int) {});
+    ok = before + need <= free;
+    if (ok)
+      scan_counts<kRowWaves>(counts, num_blocks, sums, [&](int page, int32_t, bool is_free, int r) {
+        if (is_free && r >= before && r < before + need) out[have + r - before] = page;
+      });
+  }
+  for (int j = threadIdx.x; j < t.width; j += 256)
+    if (!ok || j < have || j >= have + need) out[j] = row[j];
+  if (threadIdx.x == 0) granted[seq] = ok ? want : have_tokens;
+}
+
+__global__ __launch_bounds__(kPlanWaves* kWave) void free_small_kernel(Tables t, const int32_t* __restrict__ rows,
+                                                                       int32_t num_rows, const int32_t* __restrict__ counts,
+                                                                       int32_t num_blocks, int32_t* __restrict__ new_counts) {
+  __shared__ int named[kSmallPool];
+  for (int p = threadIdx.x; p < num_blocks; p += kPlanWaves * kWave) named[p] = 0;
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < (int64_t)num_rows * t.width; i += kPlanWaves * kWave) {
+    const int k = (int)(i / t.width), j = (int)(i - (int64_t)k * t.width), seq = rows[k];
+    if (j >= pages_of(seq_tokens(t, seq), t.block_size)) continue;
+    const int32_t page = t.tables[(int64_t)seq * t.width + j];
+    if (page >= 0 && page < num_blocks) atomicAdd(named + page, 1);
+  }
+  __syncthreads();
+  for (int p = threadIdx.x; p < num_blocks; p += kPlanWaves * kWave) new_counts[p] = max(max(counts[p], 0) - named[p], 0);
+}
+
+// As compact_kernel, with the plan in every workgroup's LDS.
+__global__ __launch_bounds__(kRowWaves* kWave) void compact_small_kernel(Tables t, const int32_t* __restrict__ counts,
+                                                                         int32_t num_blocks, Caches caches,
+                                                                         int32_t num_caches, uint32_t chunks,
+                                                                         int64_t page_elems, uint32_t row_wgs,
+                                                                         int32_t* __restrict__ new_tables,
+                                                                         int32_t* __restrict__ new_counts,
+                                                                         int32_t* __restrict__ used_out) {
+  __shared__ int sums[kRowWaves];
+  __shared__ uint16_t holes[kSmallPool / 2], movers[kSmallPool / 2];  // movers: the last one first
+  __shared__ uint16_t place[kSmallPool];                              // of a page that moves, in movers
+  __shared__ int free_below;
+  const int free = scan_counts<kRowWaves>(counts, num_blocks, sums, [](int, int32_t, bool, int) {});
+  const int used = num_blocks - free;
+  if (threadIdx.x == 0) free_below = 0;
+  scan_counts<kRowWaves>(counts, num_blocks, sums, [&](int page, int32_t, bool is_free, int rank) {
+    if (page == used) free_below = rank;
+    if (is_free && page < used) holes[rank] = (uint16_t)page;
+    if (!is_free && page >= used) {
+      const int from_end = used - 1 - (page - rank);  // used pages behind this one
+      movers[from_end] = (uint16_t)page;
+      place[page] = (uint16_t)from_end;
+    }
+  });
+  __syncthreads();
+  const int moves = free_below;
+  auto hole_of = [&](int from_end) { return (int)holes[moves - 1 - from_end]; };
+  if (blockIdx.x < row_wgs) {
+    const int64_t stride = (int64_t)row_wgs * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t entries = (int64_t)t.seqs * t.width;
+    for (int64_t i = first; i < entries; i += stride) {
+      const int seq = (int)(i / t.width), j = (int)(i - (int64_t)seq * t.width);
+      int32_t page = t.tables[i];
+      if (page >= used && page < num_blocks && j < pages_of(seq_tokens(t, seq), t.block_size) && counts[page] > 0)
+        page = hole_of(place[page]);
+      new_tables[i] = page;
+    }
+    for (int64_t p = first; p < num_blocks; p += stride) {
+      const int32_t c = counts[p];
+      if (p >= used) {
+        new_counts[p] = 0;
+        if (c > 0) new_counts[hole_of(place[p])] = c;
+      } else if (c > 0) {
+        new_counts[p] = c;
+      }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) used_out[0] = used;
+    return;
+  }
+  copy_moves(blockIdx.x - row_wgs, gridDim.x - row_wgs, moves, caches, num_caches, chunks, page_elems,
+             [&](int k) { return (int64_t)movers[k]; }, [&](int k) { return (int64_t)hole_of(k); });
 }
 
 // ------------------------------------------------------------------------------------------- host side
@@ -374,6 +620,12 @@ static PlanOut plan_layout(void* workspace, int64_t num_blocks) {
   p.movers = p.before;  // packing has no requests
   p.place = p.movers + num_blocks;
   return p;
+}
+
+// Sides of the rule: a beam step of 4 sequences in a pool of 96 pages, three calls: 17.1 us one launch each, 23.0 two
+// each; 128 children in a pool of 1024 pages 80 and 89; the largest of these calls cost as much either way.
+static bool small_pool(int64_t num_blocks, int64_t requests, int64_t max_pages) {
+  return num_blocks <= kSmallPool && requests <= kSmallEntries && requests * max_pages <= kSmallEntries;
 }
 
 static uint32_t page_chunks(int64_t page_elems) { return (uint32_t)((page_elems / 8 + kCopyPieces - 1) / kCopyPieces); }
@@ -421,11 +673,17 @@ extern "C" int aops_fork_sequences_f16(const int32_t* block_tables, const int32_
   if (!workspace || workspace_bytes < aops_pages_workspace(children, num_blocks)) return AOPS_ERR_WORKSPACE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
+  // a slice is at most four rounds of a workgroup's copy loop, unless a page is larger than 64 of them
+  const uint32_t slices = (uint32_t)std::min<int64_t>((row_elems * block_size / 8 + 4 * kCopyPieces - 1) / (4 * kCopyPieces), 64);
+  if (small_pool(num_blocks, children, max_pages)) {
+    fork_small_kernel<<<dim3((unsigned)children + 1, 1 + (unsigned)num_caches * slices), kRowWaves * kWave, 0, st>>>(
+        t, parents, (int32_t)children, c, slices, ref_counts, (int32_t)num_blocks, (uint32_t)(row_elems / 16), child_tables,
+        child_lens, new_ref_counts);
+    return record_launch_status(hipGetLastError());
+  }
   const PlanOut plan = plan_layout(workspace, num_blocks);
   pages_plan_kernel<true><<<1, kPlanWaves * kWave, 0, st>>>(t, parents, (int32_t)children, ref_counts,
                                                             (int32_t)num_blocks, new_ref_counts, plan);
-  // a slice is at most four rounds of a workgroup's copy loop, unless a page is larger than 64 of them
-  const uint32_t slices = (uint32_t)std::min<int64_t>((row_elems * block_size / 8 + 4 * kCopyPieces - 1) / (4 * kCopyPieces), 64);
   if (children > 0)
     fork_kernel<<<dim3((unsigned)children, 1 + (unsigned)num_caches * slices), 256, 0, st>>>(
         t, parents, c, slices, (int32_t)num_blocks, (uint32_t)(row_elems / 16), child_tables, child_lens, new_ref_counts,
@@ -448,6 +706,11 @@ extern "C" int aops_extend_sequences(const int32_t* block_tables, const int32_t*
   if (!workspace || workspace_bytes < aops_pages_workspace(seqs, num_blocks)) return AOPS_ERR_WORKSPACE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
+  if (small_pool(num_blocks, seqs, max_pages)) {
+    extend_small_kernel<<<(unsigned)seqs + 1, kRowWaves * kWave, 0, st>>>(t, wanted_lens, ref_counts, (int32_t)num_blocks,
+                                                                           new_tables, granted_lens, new_ref_counts);
+    return record_launch_status(hipGetLastError());
+  }
   const PlanOut plan = plan_layout(workspace, num_blocks);
   pages_plan_kernel<false><<<1, kPlanWaves * kWave, 0, st>>>(t, wanted_lens, (int32_t)seqs, ref_counts,
                                                              (int32_t)num_blocks, new_ref_counts, plan);
@@ -469,6 +732,11 @@ extern "C" int aops_free_sequences(const int32_t* block_tables, const int32_t* c
     return AOPS_ERR_INVALID_ARGUMENT;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
+  if (small_pool(num_blocks, seqs > 0 ? num_rows : 0, max_pages)) {
+    free_small_kernel<<<1, kPlanWaves * kWave, 0, st>>>(t, rows, (int32_t)(seqs > 0 ? num_rows : 0), ref_counts,
+                                                        (int32_t)num_blocks, new_ref_counts);
+    return record_launch_status(hipGetLastError());
+  }
   counts_copy_kernel<<<(unsigned)((num_blocks + 255) / 256), 256, 0, st>>>(ref_counts, (int32_t)num_blocks, new_ref_counts);
   if (num_rows > 0 && seqs > 0 && max_pages > 0)
     free_kernel<<<(unsigned)num_rows, 256, 0, st>>>(t, rows, (int32_t)num_blocks, new_ref_counts);
@@ -491,14 +759,20 @@ extern "C" int aops_compact_pages_f16(const int32_t* block_tables, const int32_t
   if (!workspace || workspace_bytes < aops_pages_workspace(0, num_blocks)) return AOPS_ERR_WORKSPACE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
-  const PlanOut plan = plan_layout(workspace, num_blocks);
-  compact_plan_kernel<<<1, kPlanWaves * kWave, 0, st>>>(ref_counts, (int32_t)num_blocks, num_used, plan);
   const int64_t page_elems = row_elems * block_size;
   const uint32_t chunks = page_chunks(page_elems);
   const int64_t ints = std::max(seqs * max_pages, num_blocks);
   const int64_t row_wgs = std::min<int64_t>(std::max<int64_t>((ints + 1023) / 1024, 1), device_cu_count());
   const int64_t most = num_blocks / 2 * num_caches * (int64_t)chunks;  // at most half of the pages move
   const int64_t copy_wgs = std::min<int64_t>(most, 8 * (int64_t)device_cu_count());
+  if (num_blocks <= kSmallPool) {
+    compact_small_kernel<<<(unsigned)(row_wgs + std::max<int64_t>(copy_wgs, 1)), kRowWaves * kWave, 0, st>>>(
+        t, ref_counts, (int32_t)num_blocks, c, (int32_t)num_caches, chunks, page_elems, (uint32_t)row_wgs, new_tables,
+        new_ref_counts, num_used);
+    return record_launch_status(hipGetLastError());
+  }
+  const PlanOut plan = plan_layout(workspace, num_blocks);
+  compact_plan_kernel<<<1, kPlanWaves * kWave, 0, st>>>(ref_counts, (int32_t)num_blocks, num_used, plan);
   compact_kernel<<<(unsigned)(row_wgs + std::max<int64_t>(copy_wgs, 1)), 256, 0, st>>>(
       t, ref_counts, (int32_t)num_blocks, c, (int32_t)num_caches, chunks, page_elems, (uint32_t)row_wgs, new_tables,
       new_ref_counts, plan);

@@ -62,7 +62,7 @@ def _dev(dev, *lists):
     return [torch.tensor(x, dtype=I, device=dev) for x in lists]
 
 
-POOLS = [(1, 16, 1, 1), (7, 16, 3, 3), (64, 16, 9, 12), (300, 32, 40, 9), (8192, 8, 200, 33), (8193, 16, 33, 40), (20000, 1, 65, 200)]
+POOLS = [(1, 16, 1, 1), (7, 16, 3, 3), (64, 16, 9, 12), (300, 32, 40, 9), (4096, 16, 60, 50), (4097, 16, 60, 50), (8192, 8, 200, 33), (8193, 16, 33, 40), (20000, 1, 65, 200)]
 
 
 @pytest.mark.parametrize("row,block,blocks,layers,pairs", [(64, 16, 9, 1, 3), (48, 7, 33, 2, 16), (1024, 128, 24, 3, 11), (16, 1, 5, 1, 2)])
@@ -164,6 +164,30 @@ def test_many_layers_and_pages_larger_than_a_copy_step(paged, dev):
     got = paged.fork_sequences(t, l, p, c, caches[:3], caches[3:])
     assert got[0].tolist() == rows and got[1].tolist() == out
     assert all(_same_bits(a, b) for a, b in zip(caches, want))
+
+
+@pytest.mark.parametrize("requests", [300, 600, 1100])
+@pytest.mark.parametrize("blocks", [700, 4096])
+def test_more_requests_than_threads(paged, dev, requests, blocks):
+    """One launch up to 16384 table entries, two beyond; pools that run dry in the middle of the requests."""
+    block, width = 4, 27
+    tables, lens, counts = _pool(requests, blocks, block, 50, width, odd=False)
+    r = random.Random(requests)
+    parents = [r.randrange(50) for _ in range(requests)]
+    ref = S.PoolRef(counts, block)
+    rows, out = ref.fork(tables, lens, parents)
+    caches = _caches(dev, blocks, 16, block, 1)
+    want = [ref.moved(x.cpu()) for x in caches]
+    t, l, p, c = _dev(dev, tables, lens, parents, counts)
+    got = paged.fork_sequences(t, l, p, c, caches[:1], caches[1:])
+    assert got[0].tolist() == rows and got[1].tolist() == out and got[2].tolist() == ref.counts
+    assert all(_same_bits(a, b) for a, b in zip(caches, want))
+    wanted = [n + r.choice([0, 1, 5, 40]) for n in out]
+    room, granted = ref.extend(rows, out, wanted)
+    more = paged.extend_sequences(got[0], got[1], _dev(dev, wanted)[0], got[2], block)
+    assert more[0].tolist() == room and more[1].tolist() == granted and more[2].tolist() == ref.counts
+    ref.free(room, granted, range(requests))
+    assert paged.free_sequences(more[0], more[1], _dev(dev, list(range(requests)))[0], more[2], block).tolist() == ref.counts
 
 
 def test_a_beam_step_in_a_graph(paged, dev):
