@@ -43,6 +43,8 @@ namespace aops {
 __host__ __device__ constexpr int chunk_waves(int head_dim) { return head_dim <= 128 ? 8 : 4; }
 __host__ __device__ constexpr int chunk_rows(int head_dim) { return 32 * chunk_waves(head_dim); }
 constexpr int kChunkUnit = 256;    // tokens per unit of the balanced partition
+constexpr int kChunkWorth = 8;     // what cutting tiles costs, in units
+constexpr int kChunkPlanHead = 4;  // ints in front of the plan: units per share
 constexpr int kChunkMaxTiles = 1024;  // of the balanced partition
 constexpr float kChunkNegBig = -1.0e30f;
 constexpr float kChunkLog2e = 1.4426950408889634f;
@@ -55,7 +57,7 @@ struct ChunkArgs {
   f16* out;
   float* lse;            // may be null
   float *part_o, *part_ml;  // partial results: [kv head][2 * shares][part_rows][D] and [..][2]
-  int32_t* plan;         // units in front of each tile (max_tiles + 1), sequence and number of each tile, tiles to join
+  int32_t* plan;         // head; units in front of each tile (max_tiles + 1), sequence and number of each tile, tiles to join
   int32_t tokens, seqs, num_heads, num_kv_heads, group, block_size, max_pages, num_blocks, window;
   int32_t max_tiles, tile_rows, shares, part_rows;  // shares: of the balanced partition, per kv head; 0: one workgroup per tile
   uint32_t block_magic, block_shift;  // x / block_size = x * magic >> shift, x < 2^31
@@ -133,7 +135,7 @@ struct ChunkDims {
   static constexpr int kJoinLds = kWaves * 16 * kStreamBlocks * kJoinBlocks * 16 * 4;
   static constexpr int kMain = kLds > kStreamLds ? (kLds > kJoinLds ? kLds : kJoinLds) : (kStreamLds > kJoinLds ? kStreamLds : kJoinLds);
   static constexpr int kSmall = 2 * kWaves * 32 * 4 + 16;         // joined maxima and sums, flags
-  static constexpr int kPlan = (3 * kChunkMaxTiles + 1) * 4;
+  static constexpr int kPlan = (3 * kChunkMaxTiles + 1 + kThreads + kWaves) * 4;
   static_assert(kMain + kSmall + kPlan <= 160 * 1024, "LDS of a CU");
 };
 
@@ -205,15 +207,15 @@ __device__ __forceinline__ float chunk_sum4(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+// Zero times a number is zero, times an infinity or NaN it is NaN.
 __device__ __forceinline__ bool chunk_not_finite(f16x8 v) {
-  const u32x4 u = __builtin_bit_cast(u32x4, v);
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    bad |= (u[i] & 0x7c00u) == 0x7c00u;
-    bad |= (u[i] & 0x7c000000u) == 0x7c000000u;
-  }
-  return bad;
+  const f16x2 zero = {0, 0};
+  f16x2 z = __builtin_shufflevector(v, v, 0, 1) * zero;
+  z += __builtin_shufflevector(v, v, 2, 3) * zero;
+  z += __builtin_shufflevector(v, v, 4, 5) * zero;
+  z += __builtin_shufflevector(v, v, 6, 7) * zero;
+  const f16 both = z[0] + z[1];
+  return both != both;
 }
 
 // Offset (in halfs) of token tok of the tile's sequence, from the start of the cache's kv head 0; entries outside the cache
@@ -489,17 +491,19 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
   auto patch = [&](int tile, int slot) {
     const int kt = k0 + tile * KT;
     if (!chunk_at_edge(a, kt, KT, t.p_first, t.p_last, t.ctx)) return;
-    bool bad = false;
+    const bool beyond = kt + my_token >= t.ctx;
 #pragma unroll
     for (int r = 0; r < kRounds; ++r)
       if ((Dims::kBlocks % kStep == 0) || my_chunk + r * kStep < Dims::kBlocks) {
         f16* at = v_ring + slot * KT * D + (threadIdx.x + r * Dims::kThreads) * 8;
-        f16x8 x = ld128(at);
-        if (kt + my_token >= t.ctx) x = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-        bad |= chunk_not_finite(x);
-        st128(at, chunk_finite(x));
+        const f16x8 x = ld128(at);
+        const bool bad = chunk_not_finite(x);
+        if (beyond) st128(at, f16x8{0, 0, 0, 0, 0, 0, 0, 0});
+        if (bad && !beyond) {
+          st128(at, chunk_finite(x));
+          flags[0] = 1;
+        }
       }
-    if (bad) flags[0] = 1;
   };
 
   // The loop is cut into a phase for the matrix core (P V of the tile before, then the scores of this one) and one for the
@@ -533,9 +537,10 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
   const f16* const k_lane = k_ring + (kg >> 1) * KT * 16 + n * 16 + (kg & 1) * 8;  // fragment s, group g: + s * 2 * KT * 16 + g * 256
   const f16* const k_half = k_ring + Dims::kFull * 2 * KT * 16 + n * 16 + (kg & 1) * 8;
   const f16* const v_lane = v_ring + lane * 4;
-  // steady: in the middle of an item, where every step issues all of its copies and no row's view ends
-  auto step = [&](auto pv, auto score, auto steady) {
+  // steady: in the middle of an item, where every step issues all of its copies; inner: where no row's view begins or ends
+  auto step = [&](auto pv, auto score, auto steady, auto inner) {
     constexpr bool kPv = decltype(pv)::value, kScore = decltype(score)::value, kSteady = decltype(steady)::value;
+    constexpr bool kInner = decltype(inner)::value;
     // slot j+n-1 = slot j-1; slot j+n-2 = slot j-2
     const int v_slot = last_slot > 0 ? last_slot - 1 : kAhead;
     if constexpr (!kSteady) {
@@ -608,10 +613,10 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
     } else {
       chunk_wait_copies<0>();
     }
-    if (!kSteady && j < tiles) patch(j, slot);
+    if (!kInner && j < tiles) patch(j, slot);
     if (second) chunk_barrier();
     if constexpr (kScore) {
-      if (!kSteady && chunk_at_edge(a, kt, KT, wp_first, wp_last, t.ctx)) chunk_mask<CB, KG>(acc, q.pos, kt, t.ctx, a.window, kg);
+      if (!kInner && chunk_at_edge(a, kt, KT, wp_first, wp_last, t.ctx)) chunk_mask<CB, KG>(acc, q.pos, kt, t.ctx, a.window, kg);
       chunk_softmax<D, CB, KG>(acc, a.scale_log2, st, p);
     }
     if (!second) chunk_barrier();
@@ -625,22 +630,22 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
   const std::false_type no;
   const int w_first = a.window > 0 ? max(chunk_window_start(wp_first, a.window) - k0, 0) / KT : 0;
   const int w_end = live && wp_last >= k0 ? min(tiles, (wp_last - k0) / KT + 1) : 0;
-  while (j <= tiles && j < min(w_first, w_end)) step(no, no, no);
+  while (j <= tiles && j < min(w_first, w_end)) step(no, no, no, no);
   if (j < w_end) {
-    step(no, yes, no);
-    // steady: every row sees the whole tile, and there are copies to issue (and room for them among the products)
+    step(no, yes, no, no);
     const int inner = a.window > 0 ? (max(chunk_window_start(t.p_last, a.window) - k0, 0) + KT - 1) / KT : 0;
-    const int outer = min(min(w_end, tiles - kAhead), max(min(t.p_first + 1, t.ctx) - k0, 0) / KT);
-    if constexpr (Dims::kBlocks * (KG / 2) + Dims::kSlices * KG >= 4 * kRounds + 4) {
-      while (j < min(w_end, inner)) step(yes, yes, no);
-      while (j < outer) step(yes, yes, yes);
+    const int outer = max(min(t.p_first + 1, t.ctx) - k0, 0) / KT, steady = min(w_end, tiles - kAhead);
+    if constexpr (Dims::kBlocks * (KG / 2) + Dims::kSlices * KG >= 4 * kRounds + 4) {  // (else no room for all copies)
+      while (j < min(steady, inner)) step(yes, yes, yes, no);
+      while (j < min(steady, outer)) step(yes, yes, yes, yes);
+      while (j < steady) step(yes, yes, yes, no);
     }
-    while (j < w_end) step(yes, yes, no);
-    step(yes, no, no);
+    while (j < w_end) step(yes, yes, no, no);
+    step(yes, no, no, no);
   }
-  while (j <= tiles) step(no, no, no);
-  ChunkArgsRef e = chunk_reread(a);
+  while (j <= tiles) step(no, no, no, no);
 
+  ChunkArgsRef e = chunk_reread(a);
 #pragma unroll
   for (int c = 0; c < CB; ++c) {
     const int r = first_row + 16 * c + n;
@@ -881,9 +886,13 @@ __global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) v
   chunk_run<D>(a, t, head, 0, t.units, -1, chunk_lds, reinterpret_cast<float*>(chunk_lds + ChunkDims<D>::kMain));
 }
 
-// Few tiles: their keys, in units of 256 tokens, are laid end to end and cut into `shares` equal shares per kv head.  A tile
-// inside one share is written directly; of the others every share leaves a partial result, in slot 2w of share w if the tile
-// began in front of the share and in slot 2w + 1 if it began in it, which chunk_merge joins in the order of the keys.
+// The same where tiles may have to be cut, which depends on the lengths: every workgroup looks at all tiles first.  Either the
+// tiles stay whole, and workgroup i of a kv head takes one of them; or their keys, in units of 256 tokens, are laid end to end
+// and cut into `shares` equal shares per kv head, one for each of the CUs.  A tile inside one share is then written directly;
+// of the others every share leaves a partial result, in slot 2w of share w if the tile began in front of the share and in slot
+// 2w + 1 if it began in it, which chunk_merge_kernel joins in the order of the keys.  The shares take kChunkWorth units longer
+// than the keys of an even distribution (30 us for full tiles: partial results, several tiles' starts and ends, the join), whole
+// tiles as long as their longest, or as their average times the rounds that the CUs need for all.
 template <int D>
 __global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) void chunk_shares_kernel(ChunkArgs) {
   ChunkArgsRef a = chunk_args();
@@ -893,80 +902,106 @@ __global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) v
   int* before = reinterpret_cast<int*>(chunk_lds + Dims::kMain + Dims::kSmall);
   int* seq = before + kChunkMaxTiles + 1;
   int* number = seq + kChunkMaxTiles;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int head = blockIdx.x % a.num_kv_heads, share_index = blockIdx.x / a.num_kv_heads;
-  // every thread: the sequence and units of its tiles
-  for (int base = 0; base < a.max_tiles; base += Dims::kThreads) {
-    const int tile = base + threadIdx.x;
-    const int first = __builtin_amdgcn_readfirstlane(tile);  // this wave's 64 tiles
-    int b = -1, index = 0, running = 0;
-    for (int64_t s0 = 0; s0 < a.seqs && running < first + kWave; s0 += kWave) {
-      int q0, n = 0;
-      if (s0 + lane < a.seqs) chunk_seq(a, (int)s0 + lane, q0, n);
-      const int mine = chunk_tiles(a, n);
-      int upto = mine;
+  int* starts = number + kChunkMaxTiles;  // first tile of each of kThreads sequences
+  int* sums = starts + Dims::kThreads;    // of the waves
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int head = blockIdx.x % a.num_kv_heads, index = blockIdx.x / a.num_kv_heads;
+  int count = 0;  // tiles
+  for (int64_t s0 = 0; s0 < a.seqs && count < a.max_tiles; s0 += Dims::kThreads) {
+    int q0, n = 0;
+    if (s0 + threadIdx.x < a.seqs) chunk_seq(a, (int)(s0 + threadIdx.x), q0, n);
+    const int mine = chunk_tiles(a, n);
+    int upto = mine;
 #pragma unroll
-      for (int d = 1; d < kWave; d <<= 1) {
-        const int o = __shfl_up(upto, d);
-        if (lane >= d) upto += o;
-      }
-      const int total = __builtin_amdgcn_readlane(upto, kWave - 1);
-      if (running + total > first) {
-        const int lanes = (int)min((int64_t)kWave, a.seqs - s0);
-        for (int k = 0; k < lanes; ++k) {
-          const int end = running + __builtin_amdgcn_readlane(upto, k), begin = end - __builtin_amdgcn_readlane(mine, k);
-          if (tile >= begin && tile < end) {
-            b = (int)s0 + k;
-            index = tile - begin;
-          }
-        }
-      }
-      running += total;
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
     }
-    if (tile < a.max_tiles) {
-      seq[tile] = b;
-      number[tile] = index;
-      before[tile + 1] = b >= 0 ? chunk_geometry(a, b, index).units : 0;
+    // (sums of bounds that overlap are cut off: nothing behind max_tiles is looked at)
+    if (lane == kWave - 1) sums[wave] = min(upto, a.max_tiles);
+    __syncthreads();
+    int in_front = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < Dims::kWaves; ++w) {
+      in_front += w < wave ? sums[w] : 0;
+      total += sums[w];
     }
+    starts[threadIdx.x] = min(in_front + upto - mine, total);
+    __syncthreads();
+    const int end = min(count + total, a.max_tiles);
+    for (int tile = count + threadIdx.x; tile < end; tile += Dims::kThreads) {
+      int k = 0;  // the last sequence that starts at or in front of the tile (those without tiles start with the next one)
+#pragma unroll
+      for (int step = Dims::kThreads / 2; step > 0; step >>= 1)
+        if (starts[k + step] <= tile - count) k += step;
+      seq[tile] = (int)s0 + k;
+      number[tile] = tile - count - starts[k];
+      before[tile + 1] = chunk_geometry(a, (int)s0 + k, tile - count - starts[k]).units;
+    }
+    count = end;
+    __syncthreads();
   }
-  __syncthreads();
   if (threadIdx.x < kWave) {  // running sums
     int running = 0;
     if (lane == 0) before[0] = 0;
-    for (int base = 0; base < a.max_tiles; base += kWave) {
-      int upto = base + lane < a.max_tiles ? before[base + lane + 1] : 0;
+    for (int base = 0; base < count; base += kWave) {
+      int upto = base + lane < count ? before[base + lane + 1] : 0;
 #pragma unroll
       for (int d = 1; d < kWave; d <<= 1) {
         const int o = __shfl_up(upto, d);
         if (lane >= d) upto += o;
       }
-      if (base + lane < a.max_tiles) before[base + lane + 1] = running + upto;
-      running += __builtin_amdgcn_readlane(upto, kWave - 1);
+      if (base + lane < count) before[base + lane + 1] = running + upto;
+      running += __shfl(upto, kWave - 1);
     }
   }
   __syncthreads();
-  if (blockIdx.x == 0) {  // for the join
-    for (int i = threadIdx.x; i <= a.max_tiles; i += Dims::kThreads) a.plan[i] = before[i];
-    for (int i = threadIdx.x; i < a.max_tiles; i += Dims::kThreads) {
-      a.plan[a.max_tiles + 1 + i] = seq[i];
-      a.plan[2 * a.max_tiles + 1 + i] = number[i];
-    }
+  count = __builtin_amdgcn_readfirstlane(count);
+  if (count == 0) {  // no sequence has a token: nothing to do, and to join
+    if (head == 0 && index < a.shares && threadIdx.x == 0) a.plan[kChunkPlanHead + 3 * a.max_tiles + 1 + index] = -1;
+    return;
   }
-  const int total = before[a.max_tiles];
-  const int share = max((total + a.shares - 1) / a.shares, 1);
-  int begin = (int)min((int64_t)share_index * share, (int64_t)total);
-  const int end = min(begin + share, total);
-  int tile = 0;
-  for (int step = kChunkMaxTiles; step > 0; step >>= 1)  // the last tile that begins at or in front of `begin`
-    if (tile + step < a.max_tiles && before[tile + step] <= begin) tile += step;
-  // for the join: the tile that this share continues, if it is the first one to do so
-  if (head == 0 && threadIdx.x == 0)
-    a.plan[3 * a.max_tiles + 1 + share_index] = begin < end && begin > before[tile] && before[tile] / share + 1 == share_index ? tile : -1;
+  const int total = __builtin_amdgcn_readfirstlane(before[count]);
+  const int share = (total + a.shares - 1) / a.shares;
+  int longest = 0;
+  for (int i = lane; i < count; i += kWave) longest = max(longest, before[i + 1] - before[i]);
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) longest = max(longest, __shfl_xor(longest, d));
+  const int rounds = (count + a.shares - 1) / a.shares;
+  const bool whole = __builtin_amdgcn_readfirstlane(max(longest, rounds * (total / count)) <= share + kChunkWorth);
+  int tile, begin, end;
+  if (whole) {
+    tile = count - 1 - index;  // the last tiles of the sequences, which see the most keys, first
+    begin = tile >= 0 ? before[tile] : 0;
+    end = tile >= 0 ? before[tile + 1] : 0;
+  } else {
+    begin = (int)min((int64_t)index * share, (int64_t)total);
+    end = index < a.shares ? min(begin + share, total) : begin;
+    tile = 0;
+#pragma unroll
+    for (int step = kChunkMaxTiles / 2; step > 0; step >>= 1)  // the last tile that begins at or in front of `begin`
+      if (tile + step < count && before[tile + step] <= begin) tile += step;
+  }
+  begin = __builtin_amdgcn_readfirstlane(begin);
+  end = __builtin_amdgcn_readfirstlane(end);
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  if (head == 0) {  // for the join: the plan, and for each share the tile that it continues, if it is the first one to do so
+    if (index == 0) {
+      for (int i = threadIdx.x; i <= count; i += Dims::kThreads) a.plan[kChunkPlanHead + i] = before[i];
+      for (int i = threadIdx.x; i < count; i += Dims::kThreads) {
+        a.plan[kChunkPlanHead + a.max_tiles + 1 + i] = seq[i];
+        a.plan[kChunkPlanHead + 2 * a.max_tiles + 1 + i] = number[i];
+      }
+      if (threadIdx.x == 0) a.plan[0] = share;
+    }
+    if (index < a.shares && threadIdx.x == 0)
+      a.plan[kChunkPlanHead + 3 * a.max_tiles + 1 + index] =
+          !whole && begin < end && begin > before[tile] && before[tile] / share + 1 == index ? tile : -1;
+  }
   while (begin < end) {
     const int from = __builtin_amdgcn_readfirstlane(before[tile]), to = __builtin_amdgcn_readfirstlane(before[tile + 1]);
     const int upto = min(end, to);
-    const bool whole = begin == from && upto == to;
-    const int part = whole ? -1 : 2 * share_index + (begin == from ? 1 : 0);
+    const int part = begin == from && upto == to ? -1 : 2 * index + (begin == from ? 1 : 0);
     ChunkArgsRef e = chunk_reread(a);
     const ChunkTile t = chunk_geometry(e, __builtin_amdgcn_readfirstlane(seq[tile]), __builtin_amdgcn_readfirstlane(number[tile]));
     chunk_run<D>(e, t, head, begin - from, upto - begin, part, chunk_lds, small);
@@ -984,7 +1019,7 @@ hipError_t chunk_launch(const ChunkArgs& a, hipStream_t stream) {
   if (a.shares > 0) {
     constexpr int lds = Dims::kMain + Dims::kSmall + Dims::kPlan;
     if (const hipError_t e = allow_dynamic_lds((const void*)chunk_shares_kernel<D>, lds, shares_done)) return e;
-    chunk_shares_kernel<D><<<(unsigned)(a.shares * a.num_kv_heads), Dims::kThreads, lds, stream>>>(a);
+    chunk_shares_kernel<D><<<(unsigned)((a.shares > a.max_tiles ? a.shares : a.max_tiles) * a.num_kv_heads), Dims::kThreads, lds, stream>>>(a);
   } else {
     constexpr int lds = Dims::kMain + Dims::kSmall;
     if (const hipError_t e = allow_dynamic_lds((const void*)chunk_tiles_kernel<D>, lds, tiles_done)) return e;

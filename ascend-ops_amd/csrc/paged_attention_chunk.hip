@@ -16,17 +16,17 @@ AOPS_CHUNK_DIMS(AOPS_CHUNK_EXTERN)
 // the many partial results of a few rows are read side by side (one after the other they took 36 us of 127 for 32 rows of
 // 32 partial results).
 constexpr int kMergeWaves = 8;
-__global__ __launch_bounds__(kMergeWaves* kWave) void chunk_merge_kernel(ChunkArgs, int head_dim, int lanes, int rows_per_wave) {
+__global__ __launch_bounds__(kMergeWaves* kWave) void chunk_merge_kernel(ChunkArgs, int head_dim, int lanes, int rows) {
   ChunkArgsRef a = chunk_args();
-  const int tile = a.plan[3 * a.max_tiles + 1 + blockIdx.z], head = blockIdx.x;
+  const int32_t* plan = a.plan + kChunkPlanHead;
+  const int tile = plan[3 * a.max_tiles + 1 + blockIdx.z], head = blockIdx.x;
   if (tile < 0) return;
-  const int from = a.plan[tile], to = a.plan[tile + 1], total = a.plan[a.max_tiles];
-  const int share = max((total + a.shares - 1) / a.shares, 1);
-  const ChunkTile t = chunk_geometry(a, a.plan[a.max_tiles + 1 + tile], a.plan[2 * a.max_tiles + 1 + tile]);
+  const int from = plan[tile], to = plan[tile + 1], share = a.plan[0];
+  const ChunkTile t = chunk_geometry(a, plan[a.max_tiles + 1 + tile], plan[2 * a.max_tiles + 1 + tile]);
   const int lane = threadIdx.x & (kWave - 1);
   const int s0 = from / share, parts = (to - 1) / share - s0 + 1;
-  const int first = (blockIdx.y * kMergeWaves + threadIdx.x / kWave) * rows_per_wave;
-  for (int r = first; r < min(first + rows_per_wave, t.rows); ++r) {
+  const int first = blockIdx.y * rows;
+  for (int r = first + threadIdx.x / kWave; r < min(first + rows, t.rows); r += kMergeWaves) {
     // the first share's part begins in that share, all others' in front of theirs
     auto slot = [&](int i) { return chunk_part_row(a, head, 2 * (s0 + i) + (i == 0 ? 1 : 0), r); };
     float ref = kChunkNegBig;
@@ -75,21 +75,17 @@ static bool chunk_sizes_ok(int64_t tokens, int64_t seqs, int64_t num_heads, int6
          tokens <= 0x3fffffff / (num_heads / num_kv_heads) && max_pages <= 0x7ffffe00 / block_size;
 }
 
-// The balanced partition pays where whole tiles would leave CUs idle: fewer than two per CU, and sequences long enough (by what a
-// row of the block table can hold) that a share is worth a partial result; and where single sequences may be so long that one
-// of their tiles would outlast all others.  (24 sequences with a window of 1024, 16 kv heads, up to 544 tiles: 74 us in whole
-// tiles, 92 balanced; 5 prompts of 77 to 2000 tokens, 656 tiles: 92 and 124; 4096 tokens over 32768 keys, 520 tiles: 1750 and
-// 1775; 16 tokens over 131079 keys, 72 tiles of which 8 exist: 114 balanced, 2.7 ms in whole tiles.)
+// Where contexts may be longer than kChunkWorth units (by what a row of the block table can hold) the kernel that can cut tiles is
+// taken, which looks at the lengths: it costs 4 us more for a small call (4 sequences of 5 tokens over up to 1004 keys: 18.7 and 22.7 us).
 static ChunkPlan chunk_plan(int64_t tokens, int64_t seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                             int64_t block_size, int64_t max_pages) {
   const int64_t group = num_heads / num_kv_heads, cus = device_cu_count(), tile_rows = chunk_rows((int)head_dim);
   ChunkPlan p = {(tokens * group + tile_rows - 1) / tile_rows + std::min(seqs, tokens), 0, 0, 16};
-  if (p.max_tiles <= kChunkMaxTiles && num_kv_heads <= cus &&
-      (p.max_tiles * num_kv_heads < 2 * cus ? max_pages * block_size > 4 * kChunkUnit : max_pages * block_size > 32 * kChunkUnit)) {
+  if (p.max_tiles <= kChunkMaxTiles && num_kv_heads <= cus && max_pages * block_size > kChunkWorth * kChunkUnit) {
     p.shares = cus / num_kv_heads;
     p.part_rows = std::min<int64_t>(tile_rows, (tokens * group + 15) / 16 * 16);
     const size_t rows = (size_t)(num_kv_heads * 2 * p.shares * p.part_rows);
-    p.bytes = rows * (size_t)(head_dim + 2) * sizeof(float) + (size_t)(3 * p.max_tiles + 1 + p.shares) * sizeof(int32_t);
+    p.bytes = rows * (size_t)(head_dim + 2) * sizeof(float) + (size_t)(kChunkPlanHead + 3 * p.max_tiles + 1 + p.shares) * sizeof(int32_t);
   }
   return p;
 }
@@ -169,9 +165,11 @@ extern "C" int aops_paged_attention_chunk_f16(const void* q, const void* key_cac
   if (e != hipSuccess || p.shares == 0) return record_launch_status(e);
   int lanes = 4;
   while (4 * lanes < head_dim) lanes *= 2;
-  const int rows_per_wave = p.part_rows <= 64 ? 1 : 4, rows = kMergeWaves * rows_per_wave;
+  // One row per wave where there are few and so, as a rule, many partial results of each (64 rows of 33: 8 us, 21 with four rows
+  // per wave), else four (80 rows, of which few need it: 6.3 us instead of 7.9, spent on workgroups that find nothing to do).
+  const int rows = p.part_rows <= 64 ? kMergeWaves : 4 * kMergeWaves;
   // (kv heads vary fastest, so that the few tiles of a small call are joined on all XCDs)
   chunk_merge_kernel<<<dim3((unsigned)num_kv_heads, (unsigned)((p.part_rows + rows - 1) / rows), (unsigned)p.shares),
-                       kMergeWaves * kWave, 0, st>>>(a, (int)head_dim, lanes, rows_per_wave);
+                       kMergeWaves * kWave, 0, st>>>(a, (int)head_dim, lanes, rows);
   return record_launch_status(hipGetLastError());
 }

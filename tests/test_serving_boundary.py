@@ -193,6 +193,6 @@ def test_c_abi_chunk_attention():
     size = lib.aops_paged_attention_chunk_workspace
     # short tables: no partial results; long ones: two slots per share, rows of the largest tile, and the plan
     assert size(4, 2, 4, 2, 64, 16, 4) == 16
-    assert size(4, 2, 4, 2, 64, 16, 400) == 2 * 2 * 128 * 16 * 66 * 4 + (3 * 3 + 1 + 128) * 4
+    assert size(4, 2, 4, 2, 64, 16, 400) == 2 * 2 * 128 * 16 * 66 * 4 + (4 + 3 * 3 + 1 + 128) * 4
     assert run(pages=400, ws_bytes=size(4, 2, 4, 2, 64, 16, 400) - 1) == -2
     assert size(4, 2, 5, 2, 64, 16, 4) == 0 and size(4, 2, 4, 2, 24, 16, 4) == 0
