@@ -254,7 +254,7 @@ __device__ __forceinline__ void chunk_load_query(ChunkArgsRef a, const ChunkTile
     const bool live = r < t.rows;
     const int row = t.row0 + (live ? r : 0);
     const int token = row / a.group;
-    q.pos[c] = live ? t.p_first + token - t.row0 / a.group : -1;
+    q.pos[c] = live ? max(t.p_first + token - t.row0 / a.group, -1) : -1;
     const f16* src = a.q + ((int64_t)(t.q0 + token) * a.num_heads + head * a.group + (row - token * a.group)) * D;
     const f16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
@@ -786,17 +786,21 @@ __device__ __forceinline__ void chunk_run_stream(ChunkArgsRef a, const ChunkTile
     for (int w = 0; w < Dims::kWaves; ++w) ref = fmaxf(ref, refs[w * 32 + 16 * c + n]);
     factor[c] = __builtin_amdgcn_exp2f(st.ref[c] - ref);
   }
-  float* acc = reinterpret_cast<float*>(lds);  // [wave][row][kJoinBlocks * 16 (+ 4, so that rows start in other banks)]
-  constexpr int kRow = Dims::kJoinBlocks * 16;
-  constexpr int kRowsAt = 16 * CB;
+  // [wave][row][four d], the groups of four d in an order that depends on the row: rows are as long as the banks are wide, so
+  // the same group of 16 rows, which a wave writes together, would fall into the same banks (12.7 us instead of 15.6 for four
+  // sequences of five tokens over up to 1004 keys)
+  f32x4* acc = reinterpret_cast<f32x4*>(lds);
+  constexpr int kRow = Dims::kJoinBlocks * 4;
+  static_assert((kRow & (kRow - 1)) == 0, "groups of a row are told apart by their bits");
+  auto at = [&](int w, int r, int g) { return (w * (16 * CB) + r) * kRow + (g ^ (r & (kRow - 1))); };
   for (int db0 = 0; db0 < Dims::kBlocks; db0 += Dims::kJoinBlocks) {
     __syncthreads();  // LDS is free: V was read, or the blocks in front of these were joined
 #pragma unroll
     for (int c = 0; c < CB; ++c)
+      if (16 * c < t.rows)
 #pragma unroll
-      for (int db = 0; db < Dims::kBlocks; ++db)
-        if (db >= db0 && db < db0 + Dims::kJoinBlocks)
-          *reinterpret_cast<f32x4*>(acc + (wave * kRowsAt + 16 * c + n) * kRow + (db - db0) * 16 + 4 * kg) = st.o[c][db] * factor[c];
+        for (int db = 0; db < Dims::kBlocks; ++db)
+          if (db >= db0 && db < db0 + Dims::kJoinBlocks) acc[at(wave, 16 * c + n, (db - db0) * 4 + kg)] = st.o[c][db] * factor[c];
     __syncthreads();
     const int width = min(Dims::kBlocks - db0, Dims::kJoinBlocks) * 4;  // groups of four d
     for (int i = threadIdx.x; i < t.rows * width; i += Dims::kThreads) {
@@ -805,7 +809,7 @@ __device__ __forceinline__ void chunk_run_stream(ChunkArgsRef a, const ChunkTile
       float ref = kChunkNegBig, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < Dims::kWaves; ++w) {
-        v += *reinterpret_cast<const f32x4*>(acc + (w * kRowsAt + r) * kRow + 4 * d4);
+        v += acc[at(w, r, d4)];
         ref = fmaxf(ref, refs[w * 32 + r]);
       }
 #pragma unroll
@@ -1009,8 +1013,6 @@ __global__ __launch_bounds__(ChunkDims<D>::kThreads, ChunkDims<D>::kWaves / 4) v
     ++tile;
   }
 }
-
-typedef hipError_t (*ChunkLaunch)(const ChunkArgs& a, hipStream_t stream);
 
 template <int D>
 hipError_t chunk_launch(const ChunkArgs& a, hipStream_t stream) {
