@@ -11,7 +11,7 @@ import ascend910a_extras.ascend910a_extras_C as _C
 
 Tensor = torch.Tensor
 
-_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "dynamic": 3, "yarn": 4, "llama3": 5, "pairs": 6}
+_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "dynamic": 3, "yarn": 4, "wavelength": 5, "pairs": 6}
 
 
 def rotary_tables(
@@ -38,7 +38,7 @@ def rotary_tables(
     ``scaling``: ``"linear"`` (``f_j / factor``), ``"ntk"`` (the base times ``factor**(R/(R-2))``), ``"dynamic"`` (the same,
     with the factor that ``max_position`` beyond ``original_max_position`` asks for), ``"yarn"`` (by parts, from
     ``beta_fast`` to ``beta_slow`` turns within ``original_max_position``; every entry times ``0.1 ln(factor) + 1``),
-    ``"llama3"`` (by wave length, between ``low_freq_factor`` and ``high_freq_factor`` turns), ``"pairs"``
+    ``"wavelength"`` (by wave length, between ``low_freq_factor`` and ``high_freq_factor`` turns), ``"pairs"``
     (``f_j / pair_factors[j]``, fp32 ``[rotary_dim/2]`` on the device; every entry times
     ``sqrt(1 + ln(factor) / ln(original_max_position))``).  ``attention_factor`` replaces the factor on the entries."""
     if scaling not in _SCALINGS:

@@ -116,7 +116,7 @@ extern "C" int aops_paged_attention_chunk_f16(const void* q, const void* key_cac
   if (max_pages > 0 && (!key_cache || !value_cache || !block_tables)) return AOPS_ERR_INVALID_ARGUMENT;
   const ChunkPlan p = chunk_plan(tokens, seqs, num_heads, num_kv_heads, head_dim, block_size, max_pages);
   if (!workspace || workspace_bytes < p.bytes) return AOPS_ERR_WORKSPACE;
-  if (p.max_tiles * num_kv_heads > 0x7fffffff) return AOPS_ERR_INVALID_ARGUMENT;
+  if (!grid_fits(p.max_tiles * num_kv_heads, kWave * chunk_waves((int)head_dim))) return AOPS_ERR_INVALID_ARGUMENT;
   // with 2^s the power of two at or above block_size, floor(2^(31+s) / block_size) + 1 is off by at most 2^s parts in
   // 2^(31+s): too little to change the quotient of a number below 2^31
   uint32_t s = 0;

@@ -645,7 +645,7 @@ extern "C" int aops_copy_pages_f16(void* const* caches, int64_t num_caches, cons
   if (!geometry_ok(num_caches, num_blocks, row_elems, block_size) || pairs < 0) return AOPS_ERR_INVALID_ARGUMENT;
   if (pairs == 0 || num_blocks == 0) return AOPS_OK;
   const uint32_t chunks = page_chunks(row_elems * block_size);
-  if (pairs > 0x7fffffff / (int64_t)chunks || !src_pages || !dst_pages) return AOPS_ERR_INVALID_ARGUMENT;
+  if (pairs > 0x7fffffff || !grid_fits(pairs * chunks, 256) || !src_pages || !dst_pages) return AOPS_ERR_INVALID_ARGUMENT;
   Caches c;
   if (const int e = fill(c, caches, num_caches)) return e;
   copy_pages_kernel<<<dim3((unsigned)(pairs * chunks), (unsigned)num_caches), 256, 0, static_cast<hipStream_t>(stream)>>>(
@@ -661,7 +661,7 @@ extern "C" int aops_fork_sequences_f16(const int32_t* block_tables, const int32_
                                        size_t workspace_bytes, void* stream) {
   using namespace aops;
   if (!geometry_ok(num_caches, num_blocks, row_elems, block_size) || !tables_ok(seqs, max_pages, block_size) ||
-      children < 0 || children > 0x7fffffff)
+      children < 0 || children > 0x7fffffff || !grid_fits(children + 1, 256))
     return AOPS_ERR_INVALID_ARGUMENT;
   if (children == 0 && num_blocks == 0) return AOPS_OK;
   if ((num_blocks > 0 && (!ref_counts || !new_ref_counts)) ||
@@ -697,7 +697,7 @@ extern "C" int aops_extend_sequences(const int32_t* block_tables, const int32_t*
                                      int32_t* granted_lens, int32_t* new_ref_counts, void* workspace,
                                      size_t workspace_bytes, void* stream) {
   using namespace aops;
-  if (!tables_ok(seqs, max_pages, block_size) || num_blocks < 0 || num_blocks >= 0x7fffffff)
+  if (!tables_ok(seqs, max_pages, block_size) || !grid_fits(seqs + 1, 256) || num_blocks < 0 || num_blocks >= 0x7fffffff)
     return AOPS_ERR_INVALID_ARGUMENT;
   if (seqs == 0 && num_blocks == 0) return AOPS_OK;
   if ((num_blocks > 0 && (!ref_counts || !new_ref_counts)) ||
@@ -723,7 +723,7 @@ extern "C" int aops_free_sequences(const int32_t* block_tables, const int32_t* c
                                    int64_t max_pages, int64_t block_size, const int32_t* rows, int64_t num_rows,
                                    const int32_t* ref_counts, int64_t num_blocks, int32_t* new_ref_counts, void* stream) {
   using namespace aops;
-  if (!tables_ok(seqs, max_pages, block_size) || num_rows < 0 || num_rows > 0x7fffffff || num_blocks < 0 ||
+  if (!tables_ok(seqs, max_pages, block_size) || num_rows < 0 || !grid_fits(num_rows, 256) || num_blocks < 0 ||
       num_blocks >= 0x7fffffff)
     return AOPS_ERR_INVALID_ARGUMENT;
   if (num_blocks == 0) return AOPS_OK;

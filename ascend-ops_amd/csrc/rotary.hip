@@ -25,14 +25,14 @@ enum RotaryScaling : int {
   kScaleNtk = 2,
   kScaleDynamic = 3,
   kScaleYarn = 4,
-  kScaleLlama3 = 5,
+  kScaleWaveLength = 5,
   kScalePairs = 6,
 };
 
 struct RotaryFreq {
   double log2_base, factor, low, high, original;
   float amplitude;
-  int kind;  // what is left to do per pair: none, linear, yarn, llama3 or pairs
+  int kind;  // what is left to do per pair: none, linear, yarn, by wave length or pairs
 };
 
 constexpr int kTableRows = 16;
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void rotary_tables_kernel(T* __restrict__ cos_
       f = f / fq.factor * ramp + f * (1.0 - ramp);
       break;
     }
-    case kScaleLlama3: {
+    case kScaleWaveLength: {
       const double turns = fq.original * f * 0.15915494309189535;  // within the original context
       if (turns < fq.low) {
         f /= fq.factor;
@@ -203,7 +203,7 @@ extern "C" int aops_rotary_tables(void* cos_out, void* sin_out, int table_fp32, 
   if (!(base > 0.0) || !isfinite(base) || !(factor > 0.0) || !isfinite(factor) || !(attention_factor >= 0.0) ||
       !isfinite(attention_factor))
     return AOPS_ERR_INVALID_ARGUMENT;
-  const bool needs_original = scaling == kScaleDynamic || scaling == kScaleYarn || scaling == kScaleLlama3 ||
+  const bool needs_original = scaling == kScaleDynamic || scaling == kScaleYarn || scaling == kScaleWaveLength ||
                               (scaling == kScalePairs && attention_factor == 0.0 && factor > 1.0);
   if (needs_original && (!(original_max_position >= 1.0) || !isfinite(original_max_position)))
     return AOPS_ERR_INVALID_ARGUMENT;
@@ -230,18 +230,18 @@ extern "C" int aops_rotary_tables(void* cos_out, void* sin_out, int table_fp32, 
     }
     case kScaleYarn: {
       // low: turns of the slowest pair that keeps its frequency (beta_fast); high: of the first that is fully divided
-      if (!(low > 0.0) || !(high > 0.0) || !isfinite(low) || !isfinite(high) || base == 1.0)
+      if (!(high > 0.0) || !(low >= high) || !isfinite(low) || !(base > 1.0))
         return AOPS_ERR_INVALID_ARGUMENT;
       auto pair_of = [&](double turns) {
         return r * log(original_max_position / (turns * kTwoPi)) / (2.0 * log(base));
       };
       fq.low = fmax(floor(pair_of(low)), 0.0);
       fq.high = fmin(ceil(pair_of(high)), r - 1.0);
-      if (fq.high == fq.low) fq.high += 0.001;
+      if (fq.high <= fq.low) fq.high = fq.low + 0.001;
       if (attention_factor == 0.0 && factor > 1.0) amplitude = 0.1 * log(factor) + 1.0;
       break;
     }
-    case kScaleLlama3:
+    case kScaleWaveLength:
       if (!(low > 0.0) || !(high > low) || !isfinite(high)) return AOPS_ERR_INVALID_ARGUMENT;
       fq.low = low;
       fq.high = high;
@@ -262,7 +262,7 @@ extern "C" int aops_rotary_tables(void* cos_out, void* sin_out, int table_fp32, 
   const int64_t half = rotary_dim / 2;
   const int64_t threads = (max_position + kTableRows - 1) / kTableRows * half;
   const int64_t grid = (threads + 255) / 256;
-  if (grid > 0x7fffffff) return AOPS_ERR_INVALID_ARGUMENT;
+  if (!grid_fits(grid, 256)) return AOPS_ERR_INVALID_ARGUMENT;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (table_fp32)
     rotary_tables_kernel<float><<<(unsigned)grid, 256, 0, st>>>(static_cast<float*>(cos_out),
@@ -280,7 +280,7 @@ extern "C" int aops_rotary_f16(const void* q, const void* k, const int32_t* posi
                                int64_t max_position, int interleaved, int64_t q_token_stride, int64_t q_head_stride,
                                int64_t k_token_stride, int64_t k_head_stride, void* stream) {
   using namespace aops;
-  if (tokens < 0 || num_heads < 0 || num_kv_heads < 0 || head_dim <= 0 || head_dim % 8 != 0 || rotary_dim < 2 ||
+  if (tokens < 0 || num_heads < 0 || num_heads > 0x7fffffff || num_kv_heads < 0 || num_kv_heads > 0x7fffffff || head_dim <= 0 || head_dim % 8 != 0 || rotary_dim < 2 ||
       rotary_dim % 2 != 0 || rotary_dim > head_dim || max_position < 0 || max_position > 0x7fffffff)
     return AOPS_ERR_INVALID_ARGUMENT;
   if (q_token_stride < 0 || q_head_stride < 0 || k_token_stride < 0 || k_head_stride < 0 || q_token_stride % 8 != 0 ||

@@ -163,10 +163,10 @@ int aops_paged_attention_chunk_f16(const void* q, const void* key_cache, const v
  *   3  the same with factor * max_position / original_max_position - (factor - 1) in the place of factor where
  *      max_position > original_max_position, and nothing changed where not
  *   4  by parts (YaRN, arXiv:2309.00071): pairs that turn more than `low` times (beta_fast, 32) within
- *      original_max_position keep f_j, pairs that turn less than `high` times (beta_slow, 1) get f_j / factor, in
- *      between (in pair numbers, rounded outwards) a linear mix
- *   5  by wave length (as Llama 3.1's configuration defines it): f_j / factor below `low` turns within
- *      original_max_position, f_j above `high` turns, a linear mix in turns in between
+ *      original_max_position keep f_j, pairs that turn less than `high` <= low times (beta_slow, 1) get f_j / factor,
+ *      in between (in pair numbers, rounded outwards) a linear mix; base > 1
+ *   5  by wave length: f_j / factor below `low` turns within original_max_position, f_j above `high` turns, a linear
+ *      mix in turns in between
  *   6  f_j / pair_factors[j], pair_factors fp32 [rotary_dim/2] on the device
  * attention_factor 0 = the scaling's own: 0.1 ln(factor) + 1 for 4, sqrt(1 + ln(factor) / ln(original_max_position))
  * for 6 (both with factor > 1), 1 otherwise.

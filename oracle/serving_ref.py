@@ -58,9 +58,9 @@ def rotary_frequencies_ref(rotary_dim, base, max_position, scaling="none", facto
         elif scaling == "yarn":
             lo = max(math.floor(r * math.log(original / (beta_fast * 2 * math.pi)) / (2 * math.log(base))), 0)
             hi = min(math.ceil(r * math.log(original / (beta_slow * 2 * math.pi)) / (2 * math.log(base))), r - 1)
-            ramp = min(max((j - lo) / ((hi - lo) or 0.001), 0.0), 1.0)
+            ramp = min(max((j - lo) / max(hi - lo, 0.001), 0.0), 1.0)
             f = f / factor * ramp + f * (1 - ramp)
-        elif scaling == "llama3":
+        elif scaling == "wavelength":
             wave = 2 * math.pi / f
             if wave > original / low:
                 f = f / factor

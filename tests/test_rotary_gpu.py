@@ -48,7 +48,8 @@ SCALINGS = [
     dict(scaling="dynamic", factor=2.0, original=5000),     # not stretched yet
     dict(scaling="yarn", factor=8.0, original=256),
     dict(scaling="yarn", factor=4.0, original=64, beta_fast=16.0, beta_slow=2.0),
-    dict(scaling="llama3", factor=8.0, original=512, low=1.0, high=4.0),
+    dict(scaling="wavelength", factor=8.0, original=512, low=1.0, high=4.0),
+    dict(scaling="yarn", factor=4.0, original=4),  # no pair turns even once: all but the first are divided
 ]
 
 

@@ -40,3 +40,58 @@ def test_no_scratch(assembly):
     for name in ("pages.hip", "rotary.hip", "paged_attention_chunk.hip"):
         sizes = re.findall(r"amdhsa_private_segment_fixed_size (\d+)", assembly[name])
         assert sizes and set(sizes) == {"0"}, name
+
+
+def _chunk_kernels(text):
+    """(kind, head size, body lines) of every chunk attention kernel."""
+    for m in re.finditer(r"^(_ZN4aops\d+chunk_(tiles|shares)_kernelILi(\d+)E\w+):[^\n]*\n(.*?)^\.Lfunc_end", text, re.S | re.M):
+        lines = (line.split(";")[0].strip() for line in m.group(4).split("\n"))
+        yield m.group(2), int(m.group(3)), [line for line in lines if line]
+
+
+def _copies_per_step(d):
+    """Fewest copies of a wave per tile of keys, the steps that may be on their way behind a counted wait, and whether all
+    waves copy the same number."""
+    tile, waves = (64 if d <= 176 else 32), (8 if d <= 128 else 4)
+    stages = 4 if 16 * tile * d <= 128 * 1024 else 3
+    chunks, per_round = d // 16, waves * 64 // (2 * tile)
+    return 2 * (chunks // per_round) + 1, stages - 2, chunks % per_round == 0
+
+
+def test_copies_to_lds_and_their_waits(assembly):
+    """The copies are assembly that the compiler does not count.  Each is its three instructions, which alone use M0; a
+    wait that leaves some on their way leaves no more than the last steps', and follows its step's copies."""
+    kernels = counted = 0
+    for name in CHUNK:
+        for kind, d, lines in _chunk_kernels(assembly[name]):
+            kernels += 1
+            where = f"chunk_{kind}_kernel<{d}>"
+            m0 = {i for i, line in enumerate(lines) if re.search(r"\bm0\b", line)}
+            for i, line in enumerate(lines):
+                if line.startswith("global_load_lds"):
+                    assert re.match(r"s_mov_b32 m0, s\d+$", lines[i - 2]) and lines[i - 1] == "s_nop 0", where
+                    m0.discard(i - 2)
+            assert not m0, (where, [lines[i] for i in sorted(m0)][:5])
+            copies, steps, all_waves_alike = _copies_per_step(d)
+            in_block = 0
+            waited = False
+            for line in lines:
+                if line.endswith(":") or line.startswith(("s_branch", "s_cbranch", "s_endpgm")):
+                    in_block, waited = 0, False
+                elif line.startswith("global_load_lds"):
+                    in_block += 1
+                    assert not waited, where  # a copy behind its step's wait would be counted with the next step's
+                elif re.match(r"s_waitcnt vmcnt\(\d+\) lgkmcnt\(0\)$", line) and in_block:
+                    n = int(re.search(r"vmcnt\((\d+)\)", line).group(1))
+                    if n:
+                        # (where only some waves copy in a step's last round, that is a branch)
+                        assert n == steps * copies and in_block >= (copies if all_waves_alike else 1), (where, n, in_block)
+                        counted += 1
+                        waited = True
+    assert kernels == 32 and counted >= 32, (kernels, counted)
+
+
+def test_tile_kernels_keep_their_registers(assembly):
+    for name in CHUNK:
+        sizes = re.findall(r"\.amdhsa_kernel _ZN4aops\d+chunk_tiles_kernel\w+\n.*?private_segment_fixed_size (\d+)", assembly[name], re.S)
+        assert len(sizes) == 4 and set(sizes) == {"0"}, name

@@ -69,7 +69,8 @@ def test_c_abi_rotary():
                 dict(factor=0.0), dict(factor=float("nan")), dict(amp=-1.0), dict(amp=float("nan")), dict(scaling=7),
                 dict(scaling=-1), dict(scaling=2, r=2), dict(scaling=3), dict(scaling=4), dict(scaling=5),
                 dict(scaling=4, orig=64.0, low=0.0), dict(scaling=4, orig=64.0, low=32.0, high=1.0, base=1.0),
-                dict(scaling=5, orig=64.0, low=4.0, high=4.0), dict(scaling=6), dict(scaling=6, factor=2.0, pairs=p),
+                dict(scaling=4, orig=64.0, low=1.0, high=32.0), dict(scaling=4, orig=64.0, low=32.0, high=1.0, base=0.5),
+                dict(n=1 << 30, r=65536), dict(scaling=5, orig=64.0, low=4.0, high=4.0), dict(scaling=6), dict(scaling=6, factor=2.0, pairs=p),
                 dict(scaling=6, factor=2.0, orig=1.0, pairs=p), dict(n=1 << 31)):
         assert tables(**bad) == -1, bad
 
@@ -79,7 +80,8 @@ def test_c_abi_rotary():
     assert embed() == 0 and embed(n=0) == 0 and embed(tokens=5, hq=0, hk=0) == 0
     for bad in (dict(tokens=-1), dict(hq=-1), dict(d=0), dict(d=60), dict(r=0), dict(r=66), dict(r=7), dict(n=-1),
                 dict(s=(4, 64, 64, 64)), dict(s=(128, -64, 64, 64)), dict(tokens=4, n=0), dict(tokens=4, ptr=None),
-                dict(tokens=1 << 31), dict(tokens=1 << 30, hq=32)):
+                dict(tokens=1 << 31), dict(tokens=1 << 30, hq=32), dict(tokens=1, hq=(1 << 63) - 1),
+                dict(tokens=1, hk=(1 << 63) - 1)):
         assert embed(**bad) == -1, bad
 
 
@@ -118,7 +120,7 @@ def test_c_abi_pages():
     assert copy() == 0 and copy(blocks=0, pairs=3) == 0
     for bad in (dict(n=0), dict(n=257), dict(pairs=-1), dict(blocks=-1), dict(row=0), dict(row=40), dict(block=0),
                 dict(pairs=2, caches=None), dict(pairs=2, caches=holes), dict(pairs=2, ptr=None),
-                dict(row=1 << 20, block=1 << 20), dict(pairs=1 << 31)):
+                dict(row=1 << 20, block=1 << 20), dict(pairs=1 << 31), dict(pairs=1 << 24), dict(pairs=(1 << 63) - 1)):
         assert copy(**bad) == -1, bad
 
     def fork(caches=many, n=2, seqs=3, width=4, children=2, blocks=8, row=64, block=16, ptr=p, ws=p, ws_bytes=1 << 20):
@@ -126,7 +128,8 @@ def test_c_abi_pages():
                                            ptr, ptr, ws, ws_bytes, None)
 
     for bad in (dict(n=0), dict(n=257), dict(seqs=-1), dict(width=-1), dict(children=-1), dict(blocks=-1), dict(row=8),
-                dict(block=0), dict(ptr=None), dict(caches=None), dict(caches=holes)):
+                dict(block=0), dict(ptr=None), dict(caches=None), dict(caches=holes), dict(children=(1 << 24) - 1),
+                dict(children=(1 << 63) - 1)):
         assert fork(**bad) == -1, bad
     assert fork(ws=None) == -2 and fork(ws_bytes=lib.aops_pages_workspace(2, 8) - 1) == -2
     assert fork(children=0, blocks=0) == 0
@@ -143,7 +146,7 @@ def test_c_abi_pages():
     def extend(seqs=3, width=4, block=16, blocks=8, ptr=p, ws=p, ws_bytes=1 << 20):
         return lib.aops_extend_sequences(ptr, ptr, ptr, seqs, width, block, ptr, blocks, ptr, ptr, ptr, ws, ws_bytes, None)
 
-    for bad in (dict(seqs=-1), dict(width=-1), dict(block=0), dict(blocks=-1), dict(ptr=None)):
+    for bad in (dict(seqs=-1), dict(width=-1), dict(block=0), dict(blocks=-1), dict(ptr=None), dict(seqs=(1 << 24) - 1)):
         assert extend(**bad) == -1, bad
     assert extend(ws=None) == -2 and extend(ws_bytes=lib.aops_pages_workspace(3, 8) - 1) == -2
     assert extend(seqs=0, blocks=0) == 0
@@ -151,7 +154,8 @@ def test_c_abi_pages():
     def free(seqs=3, width=4, block=16, rows=2, blocks=8, ptr=p):
         return lib.aops_free_sequences(ptr, ptr, seqs, width, block, ptr, rows, ptr, blocks, ptr, None)
 
-    for bad in (dict(seqs=-1), dict(width=-1), dict(block=0), dict(rows=-1), dict(blocks=-1), dict(ptr=None)):
+    for bad in (dict(seqs=-1), dict(width=-1), dict(block=0), dict(rows=-1), dict(blocks=-1), dict(ptr=None),
+                dict(rows=1 << 24)):
         assert free(**bad) == -1, bad
     assert free(blocks=0) == 0
 
@@ -187,7 +191,8 @@ def test_c_abi_chunk_attention():
     assert run(tokens=0) == 0 and run(seqs=0) == 0
     for bad in (dict(tokens=-1), dict(seqs=-1), dict(hq=0), dict(hk=0), dict(hq=5), dict(d=0), dict(d=72), dict(d=272),
                 dict(block=0), dict(pages=-1), dict(blocks=-1), dict(scale=0.0), dict(scale=float("nan")), dict(window=-1),
-                dict(ptr=None), dict(tokens=1 << 30, hq=4, hk=1), dict(tokens=1 << 31), dict(block=1 << 20, pages=1 << 20)):
+                dict(ptr=None), dict(tokens=1 << 30, hq=4, hk=1), dict(tokens=1 << 31), dict(block=1 << 20, pages=1 << 20),
+                dict(tokens=1 << 22, seqs=1 << 22)):
         assert run(**bad) == -1, bad
     assert run(ws=None) == -2
     size = lib.aops_paged_attention_chunk_workspace
