@@ -337,3 +337,64 @@ def test_two_streams_at_once(paged, dev):
                 got[i].append(paged.paged_attention_chunk(*c))
     torch.cuda.synchronize()
     assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
+
+
+@pytest.mark.parametrize("rows", [3, 60])
+@pytest.mark.parametrize("window", [0, 2700])
+def test_values_that_are_not_finite_in_cut_tiles(paged, dev, rows, window):
+    """As above where a tile's keys are shared among workgroups: at the context's end, and where the windows begin."""
+    q, kc, vc, tables, ctx, starts = _case([rows], [5000], 4, 2, 128, 16, seed=3)
+    bad = vc.clone()
+    places = [(4998, 0, 5, math.inf), (4999, 1, 6, math.nan), (2299, 0, 7, -math.inf), (2300 - rows, 1, 70, math.inf), (2298, 1, 100, math.nan)]
+    for tok, head, dim, value in places:
+        f = head * 128 + dim
+        bad[tables[0, tok // 16].long(), f // 16, tok % 16, f % 16] = value
+    o, base = (paged.paged_attention_chunk(*(t.to(dev) for t in (q, kc, v, tables, ctx, starts)), window=window).cpu() for v in (bad, vc))
+    at = torch.arange(5000 - rows, 5000)[:, None, None]
+    head, dim = torch.arange(4)[None, :, None] // 2, torch.arange(128)[None, None]
+    touched = torch.zeros(o.shape, dtype=torch.bool)
+    for tok, h, d, _ in places:
+        touched |= (head == h) & (dim == d) & (at >= tok) & ((window == 0) | (at < tok + window))
+    assert torch.equal(o[~touched], base[~touched]) and not o[touched].isfinite().any()
+
+
+def test_cut_tiles_in_two_graphs_and_on_two_streams(paged, dev):
+    """Each call has partial results of its own: graphs replayed in turn, and calls on streams at once."""
+    cases = [[t.to(dev) for t in _case(new, ctx, 4, 2, 128, 16, seed=s)] for s, (new, ctx) in enumerate([([6, 60, 1], [5000, 400, 3000]), ([40, 2], [4000, 6000])])]
+    want = [paged.paged_attention_chunk(*c, return_lse=True) for c in cases]
+    graphs, held = [], []
+    side = torch.cuda.Stream()
+    for c in cases:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            paged.paged_attention_chunk(*c, return_lse=True)
+        torch.cuda.current_stream().wait_stream(side)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(paged.paged_attention_chunk(*c, return_lse=True))
+    for i in (0, 1, 1, 0, 1, 0):
+        graphs[i].replay()
+        again = paged.paged_attention_chunk(*cases[1 - i], return_lse=True)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held[i], want[i])), i
+        assert all(torch.equal(a, b) for a, b in zip(again, want[1 - i])), i
+        for t in held[i]:
+            t.zero_()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, (s, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                got[i].append(paged.paged_attention_chunk(*c, return_lse=True))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for x in g for a, b in zip(x, w))
+
+
+@pytest.mark.parametrize("new,ctx,hq,hkv,d", [
+    ([1] * 1100, [1 + 7 * (i % 9) + (3000 if i % 400 == 3 else 0) for i in range(1100)], 2, 1, 16),  # more tiles than a partition takes
+    ([1] * 1020, [1 + 7 * (i % 9) + (3000 if i % 400 == 3 else 0) for i in range(1020)], 2, 1, 16),
+    ([0] * 700 + [2, 0, 5] + [0] * 600 + [40], [9] * 700 + [3000, 9, 70] + [0] * 600 + [2800], 2, 1, 32),  # few with tokens
+    ([2, 1], [2500, 3], 300, 300, 16),                                                                   # more kv heads than CUs
+])
+def test_long_tables_at_the_limits_of_the_partition(paged, dev, new, ctx, hq, hkv, d):
+    _check(paged, dev, _case(new, ctx, hq, hkv, d, 16))
