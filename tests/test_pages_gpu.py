@@ -190,9 +190,10 @@ def test_more_requests_than_threads(paged, dev, requests, blocks):
     assert paged.free_sequences(more[0], more[1], _dev(dev, list(range(requests)))[0], more[2], block).tolist() == ref.counts
 
 
-def test_a_beam_step_in_a_graph(paged, dev):
+@pytest.mark.parametrize("blocks", [60, 4200])
+def test_a_beam_step_in_a_graph(paged, dev, blocks):
     """Fork, extend, free and pack captured once, on one stream, and replayed on pools that change in place."""
-    blocks, block, seqs, width = 60, 16, 5, 8
+    block, seqs, width = 16, 5, 8
     state = _dev(dev, *_pool(0, blocks, block, seqs, width, odd=False))
     parents, rows_all = _dev(dev, [0, 0, 3, 1], list(range(seqs)))
     caches = _caches(dev, blocks, 32, block, 1)
@@ -236,3 +237,27 @@ def test_a_beam_step_in_a_graph(paged, dev):
         packed, used = ref.compact(room, granted)
         assert [x.tolist() for x in got] == [rows, out, room, granted, packed, ref.counts, [used]]
         assert _same_bits(after[0], ref.moved(first))
+
+
+@pytest.mark.parametrize("blocks", [60, 4200])
+def test_two_streams_at_once(paged, dev, blocks):
+    """Two pools' calls side by side."""
+    pools = [_dev(dev, *_pool(s, blocks, 16, 5, 8, odd=False)) for s in (0, 1)]
+    caches = [_caches(dev, blocks, 32, 16, 1, seed=s) for s in (0, 1)]
+    parents, wanted = _dev(dev, [0, 0, 3, 1], [100] * 5)
+
+    def step(i):
+        t, l, c = pools[i]
+        rows, lens, counts = paged.fork_sequences(t, l, parents, c, caches[i][:1], caches[i][1:])
+        counts = paged.free_sequences(rows, lens, parents, counts, 16)
+        return [rows, lens, counts, *paged.extend_sequences(t, l, wanted, c, 16)]
+
+    want = [step(i) for i in (0, 1)]
+    streams, got = [torch.cuda.Stream() for _ in pools], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for x in g for a, b in zip(x, w))

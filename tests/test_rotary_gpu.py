@@ -168,3 +168,28 @@ def test_types_and_devices_are_checked(rotary, dev):
         rotary.rotary_tables(4, 64, scaling="pairs", pair_factors=torch.ones(31, device=dev))
     with pytest.raises(RuntimeError, match="invalid argument"):
         rotary.rotary_tables(4, 64, base=-1.0, device=dev)
+
+
+def test_in_a_graph_and_on_another_stream(rotary, dev):
+    q, k = torch.randn(40, 4, 64).half().to(dev), torch.randn(40, 2, 64).half().to(dev)
+    pos = torch.arange(40, dtype=torch.int32, device=dev)
+
+    def step():
+        cos, sin = rotary.rotary_tables(300, 48, scaling="dynamic", factor=2.0, original_max_position=100, device=dev)
+        return [cos, sin, *rotary.rotary_embedding(q, k, pos, cos, sin), *rotary.rotary_embedding(q, k, pos, cos, sin, interleaved=True)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(first, step()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        q.copy_(torch.randn(40, 4, 64).half())
+        pos.add_(60)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, step())), i
