@@ -78,6 +78,7 @@ __device__ __forceinline__ ChunkArgsRef chunk_reread(ChunkArgsRef a) {
 // A tile: rows row0 + rows - 1 of sequence b's (token, head) rows.
 struct ChunkTile {
   int b, q0, row0, rows;
+  bool alone;           // the only one of its sequence
   int p_first, p_last;  // positions of its first and last row's tokens (may be negative: sees nothing)
   int ctx;              // keys there are
   int lo, hi;           // keys seen by any of its rows
@@ -103,6 +104,7 @@ __device__ __forceinline__ ChunkTile chunk_geometry(ChunkArgsRef a, int b, int i
   chunk_seq(a, b, t.q0, n);
   // the sequence's rows in even tiles (whole waves of 32): a nearly empty last one would take as long as a full one
   const int tiles = chunk_tiles(a, n), per = ((n * a.group + tiles - 1) / tiles + 31) & ~31;
+  t.alone = tiles == 1;
   t.row0 = index * per;
   t.rows = min(n * a.group - t.row0, per);
   const int len = max(a.context_lens[b], 0);
@@ -144,10 +146,15 @@ __device__ __forceinline__ uint32_t chunk_lds_address(const void* p) {
 }
 
 // 16 bytes per lane from memory to LDS, lane l's to to + 16 l.  M0 carries the address; nothing else in these kernels uses it.
+// ONCE: of lines that nobody else will read, which need not stay in the caches.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+template <bool ONCE>
 __device__ __forceinline__ void chunk_copy16(const f16* from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(to), "v"(from) : "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0");
 }
 __device__ __forceinline__ void chunk_copy4(const int32_t* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "m0");
@@ -438,18 +445,22 @@ __device__ void chunk_add_not_finite(ChunkArgsRef a, const ChunkTile& t, int hea
     }
 }
 
-// Keys k0 .. k1-1 (k0 a multiple of the tile) for a tile of many rows.
-template <int D>
+// Keys k0 .. k1-1 (k0 a multiple of the tile) for a tile of many rows.  ONCE: no other tile reads these keys.  SPLIT, for at most
+// half of the rows that a tile may have: the second half of the waves has the rows of the first one again, and every wave takes
+// one half of each tile's keys.
+template <int D, bool ONCE, bool SPLIT>
 __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& t, int head, int k0, int k1, int part,
                                                unsigned char* lds, int* flags) {
   using Dims = ChunkDims<D>;
-  constexpr int KT = Dims::kTile, KG = KT / 16, CB = 2;
+  constexpr int KT = Dims::kTile, KG = KT / (SPLIT ? 32 : 16), CB = 2;  // KG: a wave's groups of 16 keys per tile
+  constexpr int kRowWaves = Dims::kWaves / (SPLIT ? 2 : 1);
   constexpr int kPieces = 2 * KT;                       // 16-byte pieces of one chunk of a tile
   constexpr int kStep = Dims::kThreads / kPieces;       // chunks per round of the workgroup
   constexpr int kRounds = (Dims::kBlocks + kStep - 1) / kStep;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x & (kWave - 1), n = lane & 15, kg = lane >> 4;
-  const int first_row = 32 * wave;
+  const int first_row = 32 * (wave % kRowWaves);
+  const int key0 = wave / kRowWaves * (KT / 2);  // first key of a tile that is this wave's (not SPLIT: 0)
   const bool live = first_row < t.rows;
 
   ChunkQuery<D, CB> q;
@@ -481,7 +492,7 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
   };
   auto copy_round = [&](const f16* cache, int64_t off, uint32_t ring, int slot, int r) {
     if ((Dims::kBlocks % kStep == 0) || my_chunk + r * kStep < Dims::kBlocks)
-      chunk_copy16(cache + off + r * kStep * chunk_elems, ring + slot * (KT * D * 2) + r * (Dims::kThreads * 16));
+      chunk_copy16<ONCE>(cache + off + r * kStep * chunk_elems, ring + slot * (KT * D * 2) + r * (Dims::kThreads * 16));
   };
   auto copy = [&](const f16* cache, int64_t off, uint32_t ring, int slot) {
 #pragma unroll
@@ -534,9 +545,11 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
 
   f16x8 p[CB][KG / 2];
   int j = 0, slot = 0, last_slot = Dims::kStages - 1;  // of K(j) and V(j), and of K(j-1) and V(j-1)
-  const f16* const k_lane = k_ring + (kg >> 1) * KT * 16 + n * 16 + (kg & 1) * 8;  // fragment s, group g: + s * 2 * KT * 16 + g * 256
-  const f16* const k_half = k_ring + Dims::kFull * 2 * KT * 16 + n * 16 + (kg & 1) * 8;
-  const f16* const v_lane = v_ring + lane * 4;
+  constexpr int kFragments = Dims::kBlocks * (KG / 2) + Dims::kSlices * KG;  // of a step
+  constexpr int kEvery = kFragments >= 4 * kRounds + 4 ? 2 : 1;              // a copy behind each so many-th
+  const f16* const k_lane = k_ring + (kg >> 1) * KT * 16 + (key0 + n) * 16 + (kg & 1) * 8;  // fragment s, group g: + s * 2 * KT * 16 + g * 256
+  const f16* const k_half = k_ring + Dims::kFull * 2 * KT * 16 + (key0 + n) * 16 + (kg & 1) * 8;
+  const f16* const v_lane = v_ring + key0 * 16 + lane * 4;
   // steady: in the middle of an item, where every step issues all of its copies; inner: where no row's view begins or ends
   auto step = [&](auto pv, auto score, auto steady, auto inner) {
     constexpr bool kPv = decltype(pv)::value, kScore = decltype(score)::value, kSteady = decltype(steady)::value;
@@ -551,10 +564,11 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
         copy_page(j + 2 * kAhead);  // (behind the last tile: of the last token, and not used)
       }
     }
-    const int kt = k0 + j * KT;
+    const int kt = k0 + j * KT + key0;
     f32x4 acc[CB][KG];
     // Fragments of V (two reads each), then of K (one), each for CB products; a fragment is read kRing fragments before its
-    // products, and a steady step issues a copy behind every second one, where the matrix core is busy.  The order is the one
+    // products, and a steady step issues a copy behind every second one (or, if they are too few, every one), where the matrix core
+    // is busy.  The order is the one
     // written here: left to itself the compiler reads each fragment right in front of its products and waits for LDS, and
     // copies in front of them all would leave the matrix core idle.
     constexpr int kRing = 4, kV = kPv ? Dims::kBlocks * (KG / 2) : 0, kK = kScore ? Dims::kSlices * KG : 0;
@@ -589,8 +603,8 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
     };
     auto copies = [&](auto at) {
       constexpr int I = decltype(at)::value;
-      if constexpr (kSteady && I % 2 == 1) {
-        constexpr int R = I / 2;
+      if constexpr (kSteady && I % kEvery == kEvery - 1) {
+        constexpr int R = I / kEvery;
         if constexpr (R < kRounds) copy_round(a.value_cache, off_v, v_to, v_slot, R);
         if constexpr (R == kRounds) off_v = offset_of(j + kAhead);
         if constexpr (R > kRounds && R <= 2 * kRounds) copy_round(a.key_cache, off_v, k_to, last_slot, R - kRounds - 1);
@@ -616,7 +630,7 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
     if (!kInner && j < tiles) patch(j, slot);
     if (second) chunk_barrier();
     if constexpr (kScore) {
-      if (!kInner && chunk_at_edge(a, kt, KT, wp_first, wp_last, t.ctx)) chunk_mask<CB, KG>(acc, q.pos, kt, t.ctx, a.window, kg);
+      if (!kInner && chunk_at_edge(a, kt, 16 * KG, wp_first, wp_last, t.ctx)) chunk_mask<CB, KG>(acc, q.pos, kt, t.ctx, a.window, kg);
       chunk_softmax<D, CB, KG>(acc, a.scale_log2, st, p);
     }
     if (!second) chunk_barrier();
@@ -635,7 +649,7 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
     step(no, yes, no, no);
     const int inner = a.window > 0 ? (max(chunk_window_start(t.p_last, a.window) - k0, 0) + KT - 1) / KT : 0;
     const int outer = max(min(t.p_first + 1, t.ctx) - k0, 0) / KT, steady = min(w_end, tiles - kAhead);
-    if constexpr (Dims::kBlocks * (KG / 2) + Dims::kSlices * KG >= 4 * kRounds + 4) {  // (else no room for all copies)
+    if constexpr (kFragments >= 2 * kRounds + 2) {  // (else no room for all copies)
       while (j < min(steady, inner)) step(yes, yes, yes, no);
       while (j < min(steady, outer)) step(yes, yes, yes, yes);
       while (j < steady) step(yes, yes, yes, no);
@@ -646,11 +660,37 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
   while (j <= tiles) step(no, no, no, no);
 
   ChunkArgsRef e = chunk_reread(a);
+  static_assert(!SPLIT || (KG == 2 && kRowWaves * CB * (Dims::kBlocks + 1) * kWave * 16 <= Dims::kMain), "halves of a tile, and room");
+  if constexpr (SPLIT) {  // the second half's results join those of the wave with the same rows
+    f32x4* const out = reinterpret_cast<f32x4*>(lds) + (wave % kRowWaves) * (CB * (Dims::kBlocks + 1) * kWave) + lane;
+    __syncthreads();  // the last tile has been read
+    if (wave >= kRowWaves) {
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+#pragma unroll
+        for (int db = 0; db < Dims::kBlocks; ++db) out[(c * (Dims::kBlocks + 1) + db) * kWave] = st.o[c][db];
+        out[(c * (Dims::kBlocks + 1) + Dims::kBlocks) * kWave] = f32x4{st.ref[c], st.sum[c], 0.f, 0.f};
+      }
+    }
+    __syncthreads();
+    if (wave < kRowWaves) {
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        const f32x4 other = out[(c * (Dims::kBlocks + 1) + Dims::kBlocks) * kWave];
+        const float ref = fmaxf(st.ref[c], other[0]);
+        const float mine = __builtin_amdgcn_exp2f(st.ref[c] - ref), theirs = __builtin_amdgcn_exp2f(other[0] - ref);
+        st.ref[c] = ref;
+        st.sum[c] = st.sum[c] * mine + other[1] * theirs;
+#pragma unroll
+        for (int db = 0; db < Dims::kBlocks; ++db) st.o[c][db] = st.o[c][db] * mine + out[(c * (Dims::kBlocks + 1) + db) * kWave] * theirs;
+      }
+    }
+  }
 #pragma unroll
   for (int c = 0; c < CB; ++c) {
     const int r = first_row + 16 * c + n;
     const float sum = chunk_sum4(st.sum[c]);
-    if (r >= t.rows) continue;
+    if (r >= t.rows || (SPLIT && wave >= kRowWaves)) continue;
     if (part < 0) {
       const int64_t row = chunk_out_row<D>(e, t, head, r);
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
@@ -844,7 +884,22 @@ __device__ __forceinline__ void chunk_run(ChunkArgsRef a, const ChunkTile& t, in
     chunk_run_stream<D>(a, t, head, k0, k1, part, lds, small);
   } else {
     const int first = max(k0, t.lo / ChunkDims<D>::kTile * ChunkDims<D>::kTile);
-    chunk_run_tile<D>(a, t, head, first, k1, part, lds, reinterpret_cast<int*>(small));
+    int* const flags = reinterpret_cast<int*>(small);
+    // Keys that one tile reads go past the caches (64 rows over 131079 keys: 100 us instead of 112; those that four tiles
+    // read 318 instead of 294).  Halves of the waves with a half of the keys each where a whole tile is one workgroup's, whose
+    // time is that of its steps (16 sequences of 100 rows over 3000 keys, 8 heads: 60 us instead of 73), not where tiles are cut
+    // and all CUs wait for memory (8 of 128 rows over 8000 keys: 84 us, not split 74-79).
+    if (!t.alone) {
+      chunk_run_tile<D, false, false>(a, t, head, first, k1, part, lds, flags);
+      return;
+    }
+    if constexpr (ChunkDims<D>::kTile == 64) {
+      if (part < 0 && t.rows <= chunk_rows(D) / 2) {
+        chunk_run_tile<D, true, true>(a, t, head, first, k1, part, lds, flags);
+        return;
+      }
+    }
+    chunk_run_tile<D, true, false>(a, t, head, first, k1, part, lds, flags);
   }
 }
 

@@ -398,3 +398,12 @@ def test_cut_tiles_in_two_graphs_and_on_two_streams(paged, dev):
 ])
 def test_long_tables_at_the_limits_of_the_partition(paged, dev, new, ctx, hq, hkv, d):
     _check(paged, dev, _case(new, ctx, hq, hkv, d, 16))
+
+
+@pytest.mark.parametrize("d", [16, 80, 128, 144, 208])
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("new,ctx", [([33, 1, 64], [33, 400, 290]), ([65, 128], [333, 128]), ([129, 192], [129, 500]), ([256, 257], [700, 300]),
+                                     ([96, 100], [3100, 2900])])
+def test_tiles_of_every_height(paged, dev, d, window, new, ctx):
+    """Around the numbers of rows at which a tile's work is divided differently."""
+    _check(paged, dev, _case(new, ctx, 1, 1, d, 16, seed=d), window=window)
