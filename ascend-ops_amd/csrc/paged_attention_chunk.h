@@ -9,7 +9,8 @@
 // one per CU, runs over the keys a tile sees, once, with the running maximum and sum of its softmax in registers.
 //
 //  * More than 32 rows ("tile"): wave w owns rows 32w .. 32w+31, in two blocks of 16 columns; the waves
-//    share K and V tiles of kTile tokens in LDS, which are on their way while others are computed.
+//    share K and V tiles of kTile tokens in LDS, which are on their way while others are computed.  Tiles of at most half the
+//    rows may give each half of the waves one half of every tile's keys instead (chunk_run).
 //  * Fewer ("stream", the decode-like case): every wave owns all rows and its own 32 tokens of every 256 (128); K goes from
 //    memory straight into the operand registers, V through the wave's own piece of LDS, no barriers in the loop, and the
 //    eight waves are joined through LDS at the end.
@@ -30,6 +31,17 @@
 // are zeroed on the way in; a V row that some rows of the tile see and others must not, and that holds an infinity or NaN,
 // would spread through the product as 0 * inf, so tiles at an edge of the mask are searched for such values, which are left out
 // of the products and added to the results (chunk_add_not_finite).
+//
+// What it measured (MI355X; 32 query and 8 kv heads of 128 elements, pages of 128 tokens unless said otherwise):
+//    4096 tokens over 32768 keys   1720-1800 us over the cards seen, 1.15-1.20 PFLOP/s (a library matrix product of 8192^3 reached
+//                                  1.47): bound by the matrix core under the power limit (1.9 GHz; busy 0.59 of the cycles; the same
+//                                  loop with the softmax left out takes 1250 us)
+//    16 tokens over 131079 keys    98 us, 5.5 TB/s of K and V (a copy of 1 GiB reached 5.0 read and written): bound by HBM, 90 us,
+//                                  and by joining partial results
+//    24 sequences, 14 of one token and 10 of 253 to 470, window 1024, 16 + 16 heads of 80, pages of 16 tokens
+//                                  86 us: 304 tiles and 224 single rows on 256 CUs, two rounds of about 40 us of 20 steps each
+//    4 sequences of 2 to 5 tokens over up to 704 keys   12.7 us: latency, four steps of about 1.2 us on 32 CUs between 3 us that
+//                                  find and load the rows and 3 us that join and store them
 #pragma once
 
 #include <type_traits>
@@ -515,17 +527,19 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
           flags[0] = 1;
         }
       }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // written before the barrier that follows, which waits for nothing itself
   };
 
-  // The loop is cut into a phase for the matrix core (P V of the tile before, then the scores of this one) and one for the
-  // vector units (the softmax), with a barrier behind each, and waves 4-7, which share their SIMDs with waves 0-3, run one
-  // phase behind these: while one wave of a SIMD keeps the matrix core busy the other one computes weights.
-  //   phase 2j: waves 0-3 P V(j-1), S(j), waves 4-7 softmax(j-1);  phase 2j+1: waves 4-7 P V(j-1), S(j), waves 0-3 softmax(j)
-  // K and V go straight to LDS, in rings of n = kStages tiles each.  At the start of its phase for tile j a wave issues its copies
-  // for K(j+n-1) and V(j+n-2), into the slots of K(j-1) and V(j-2), which waves 4-7 read last, in phase 2j-1, and for the page
-  // numbers of tile j+2n-2.  At the end of that phase it waits for all but those of the last n-2 tiles: K(j+1) and V(j), first
-  // read in phase 2j+2, behind the barriers of both halves, and the page numbers of tile j+n, read at its next phase's start,
-  // have then arrived.
+  // A step is work for the matrix core (P V of the tile before, then the scores of this one) and then for the vector units (the
+  // softmax), with one barrier: waves 0-3 meet it behind their softmax, waves 4-7, which share their SIMDs with these, behind
+  // their products, so that they run half a step behind them: while one wave of a SIMD keeps the matrix core busy the other one
+  // computes weights (4096 tokens over 32768 keys: 1787 us, 1883 with a barrier behind each half, 2935 when all waves did the
+  // same at the same time and waited for their copies).
+  // K and V go straight to LDS, in rings of n = kStages tiles each.  At the start of its step for tile j a wave issues its copies
+  // for K(j+n-1) and V(j+n-2), into the slots of K(j-1) and V(j-2), which all waves have read in front of the barrier that they
+  // met last, and for the page numbers of tile j+2n-2.  In front of its barrier it waits for all but those of the last n-2
+  // tiles: K(j+1) and V(j), which waves read in their step j+1, and the page numbers of tile j+n, read at that step's start, have then
+  // arrived.
   // The copies are assembly that the compiler does not count (it would turn every wait for an LDS read into a wait for all of
   // them); a wave issues at least kCopies per tile.
   constexpr int kAhead = Dims::kStages - 1, kCopies = 2 * (Dims::kBlocks / kStep) + 1;
@@ -568,8 +582,7 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
     f32x4 acc[CB][KG];
     // Fragments of V (two reads each), then of K (one), each for CB products; a fragment is read kRing fragments before its
     // products, and a steady step issues a copy behind every second one (or, if they are too few, every one), where the matrix core
-    // is busy.  The order is the one
-    // written here: left to itself the compiler reads each fragment right in front of its products and waits for LDS, and
+    // is busy.  The order is the one written here: left to itself the compiler reads each fragment right in front of its products and waits for LDS, and
     // copies in front of them all would leave the matrix core idle.
     constexpr int kRing = 4, kV = kPv ? Dims::kBlocks * (KG / 2) : 0, kK = kScore ? Dims::kSlices * KG : 0;
     f16x8 ring[kRing];

@@ -91,6 +91,23 @@ def test_copies_to_lds_and_their_waits(assembly):
     assert kernels == 32 and counted >= 32, (kernels, counted)
 
 
+def test_lds_is_written_before_a_barrier(assembly):
+    """The barriers of the loops are bare: a wave waits for its own LDS writes in front of them."""
+    barriers = 0
+    for name in CHUNK:
+        for kind, d, lines in _chunk_kernels(assembly[name]):
+            pending = None
+            for line in lines:
+                if line.startswith("ds_write"):
+                    pending = line
+                elif line.startswith("s_waitcnt") and "lgkmcnt(0)" in line:
+                    pending = None
+                elif line == "s_barrier":
+                    barriers += 1
+                    assert pending is None, (f"chunk_{kind}_kernel<{d}>", pending)
+    assert barriers > 500
+
+
 def test_tile_kernels_keep_their_registers(assembly):
     for name in CHUNK:
         sizes = re.findall(r"\.amdhsa_kernel _ZN4aops\d+chunk_tiles_kernel\w+\n.*?private_segment_fixed_size (\d+)", assembly[name], re.S)
