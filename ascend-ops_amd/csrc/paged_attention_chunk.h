@@ -313,7 +313,7 @@ __device__ __forceinline__ void chunk_mask(f32x4 (&s)[CB][KG], const int (&pos)[
   }
 }
 
-// Scores as the matrix core left them.  Its results may be read six wait states after it (four passes and two); the
+// Scores as the matrix core left them.  Its results may be read only some wait states after it (four passes and a few); the
 // compiler cannot tell for the assembly that reads them below, so the wait is part of handing them over.
 template <int CB, int KG>
 __device__ __forceinline__ void chunk_settle(f32x4 (&acc)[CB][KG]) {

@@ -199,5 +199,6 @@ def test_c_abi_chunk_attention():
     # short tables: no partial results; long ones: two slots per share, rows of the largest tile, and the plan
     assert size(4, 2, 4, 2, 64, 16, 4) == 16
     assert size(4, 2, 4, 2, 64, 16, 400) == 2 * 2 * 128 * 16 * 66 * 4 + (4 + 3 * 3 + 1 + 128) * 4
+    assert size(100000, 1, 2, 1, 128, 1 << 16, 32767) == 16  # the partition counts in 32 bits
     assert run(pages=400, ws_bytes=size(4, 2, 4, 2, 64, 16, 400) - 1) == -2
     assert size(4, 2, 5, 2, 64, 16, 4) == 0 and size(4, 2, 4, 2, 24, 16, 4) == 0
