@@ -533,8 +533,8 @@ __device__ __forceinline__ void chunk_run_tile(ChunkArgsRef a, const ChunkTile& 
   // A step is work for the matrix core (P V of the tile before, then the scores of this one) and then for the vector units (the
   // softmax), with one barrier: waves 0-3 meet it behind their softmax, waves 4-7, which share their SIMDs with these, behind
   // their products, so that they run half a step behind them: while one wave of a SIMD keeps the matrix core busy the other one
-  // computes weights (4096 tokens over 32768 keys: 1787 us, 1883 with a barrier behind each half, 2935 when all waves did the
-  // same at the same time and waited for their copies).
+  // computes weights (4096 tokens over 32768 keys: 1787 us, 1883 with a barrier behind each half, 2935 in a first
+  // version, whose waves all did the same at the same time).
   // K and V go straight to LDS, in rings of n = kStages tiles each.  At the start of its step for tile j a wave issues its copies
   // for K(j+n-1) and V(j+n-2), into the slots of K(j-1) and V(j-2), which all waves have read in front of the barrier that they
   // met last, and for the page numbers of tile j+2n-2.  In front of its barrier it waits for all but those of the last n-2
