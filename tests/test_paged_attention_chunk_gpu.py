@@ -394,6 +394,7 @@ def test_cut_tiles_in_two_graphs_and_on_two_streams(paged, dev):
     ([1] * 1100, [1 + 7 * (i % 9) + (3000 if i % 400 == 3 else 0) for i in range(1100)], 2, 1, 16),  # more tiles than a partition takes
     ([1] * 1020, [1 + 7 * (i % 9) + (3000 if i % 400 == 3 else 0) for i in range(1020)], 2, 1, 16),
     ([0] * 700 + [2, 0, 5] + [0] * 600 + [40], [9] * 700 + [3000, 9, 70] + [0] * 600 + [2800], 2, 1, 32),  # few with tokens
+    ([1, 3, 40], [500, 2600, 3000], 300, 1, 16),                                                          # a token's heads in more than one tile
     ([2, 1], [2500, 3], 300, 300, 16),                                                                   # more kv heads than CUs
 ])
 def test_long_tables_at_the_limits_of_the_partition(paged, dev, new, ctx, hq, hkv, d):
