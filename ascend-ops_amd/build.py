@@ -24,7 +24,19 @@ OUT_DIR = HERE / "ascend910a_extras"
 LIB_NAME = "libaops.so"
 ARCH = "gfx950"
 
+# (those that take the compiler longest first)
 SOURCES = [
+    "paged_attention.hip",
+    "grouped_matmul_persistent.hip",
+    "grouped_matmul_tiles.hip",
+    "paged_attention_chunk_d0.hip",
+    "paged_attention_chunk_d1.hip",
+    "paged_attention_chunk_d2.hip",
+    "paged_attention_chunk_d3.hip",
+    "paged_attention_chunk_d4.hip",
+    "paged_attention_chunk_d5.hip",
+    "paged_attention_chunk_d6.hip",
+    "paged_attention_chunk_d7.hip",
     "aops_api.hip",
     "add_rms_norm.hip",
     "swiglu.hip",
@@ -34,15 +46,8 @@ SOURCES = [
     "pages.hip",
     "moe.hip",
     "reshape_and_cache.hip",
-    "paged_attention.hip",
     "paged_attention_chunk.hip",
-    "paged_attention_chunk_d0.hip",
-    "paged_attention_chunk_d1.hip",
-    "paged_attention_chunk_d2.hip",
-    "paged_attention_chunk_d3.hip",
     "grouped_matmul.hip",
-    "grouped_matmul_tiles.hip",
-    "grouped_matmul_persistent.hip",
     "matmul_fewrows.hip",
     "probes.hip",
 ]

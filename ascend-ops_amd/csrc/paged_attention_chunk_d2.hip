@@ -1,9 +1,7 @@
-// Instantiations of the chunk attention kernels, four head sizes to a file so that the build is spread over the CPUs.
+// Instantiations of the chunk attention kernels, two head sizes to a file so that the build is spread over the CPUs.
 #include "paged_attention_chunk.h"
 
 namespace aops {
-template hipError_t chunk_launch<112>(const ChunkArgs&, hipStream_t);
-template hipError_t chunk_launch<128>(const ChunkArgs&, hipStream_t);
-template hipError_t chunk_launch<144>(const ChunkArgs&, hipStream_t);
+template hipError_t chunk_launch<48>(const ChunkArgs&, hipStream_t);
 template hipError_t chunk_launch<224>(const ChunkArgs&, hipStream_t);
 }  // namespace aops
