@@ -374,46 +374,46 @@ __global__ __launch_bounds__(256) void compact_kernel(Tables t, const int32_t* _
 }
 
 // ------------------------------------------------------------------------------------------- small pools
-// The same operators in one launch, for pools of up to kSmallPool pages and tables of up to kSmallEntries entries: a decode
-// step's calls, where each launch counts (about 2 us on the host and as much between two kernels).  Every workgroup finds what it
+// The same operators in one launch, for pools of up to kSmallPool pages, up to kSmallRequests requests (one per thread) and
+// tables of up to kSmallEntries entries: a decode step's calls, where each launch counts (about 2 us on the host and as much between two kernels).  Every workgroup finds what it
 // needs of the plan itself, from counts that are a few KiB in the L2, and one workgroup makes the new counts, in LDS.
 constexpr int kSmallPool = 4096;
+constexpr int kSmallRequests = kRowWaves * kWave;
 constexpr int64_t kSmallEntries = 16384;
 
 // Pages asked for by the requests in front of request i; called by a workgroup of kRowWaves waves.
 template <bool FORK>
 __device__ __forceinline__ int asked_before(const Tables& t, const int32_t* who, int i, int* sums) {
-  int64_t mine = 0;
-  for (int k = threadIdx.x; k < i; k += kRowWaves * kWave) mine += plan_request<FORK>(t, who, k);
-  return workgroup_sum<kRowWaves>((int)min(mine, (int64_t)kSmallPool + 1), sums);
+  const int k = threadIdx.x;
+  return workgroup_sum<kRowWaves>(k < i ? min(plan_request<FORK>(t, who, k), kSmallPool + 1) : 0, sums);
 }
 
-// Pages given out: the largest sum of leading requests that the free pages suffice for.
+// Pages asked for by this thread's request and those in front of it.
 template <bool FORK>
-__device__ __forceinline__ int given_out(const Tables& t, const int32_t* who, int requests, int free, int* sums) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int asked = 0, given = 0;
-  for (int64_t tile = 0; tile < requests; tile += kRowWaves * kWave) {
-    const int64_t i = tile + threadIdx.x;
-    int upto = i < requests ? min(plan_request<FORK>(t, who, (int)i), kSmallPool + 1) : 0;
+__device__ __forceinline__ int asked_upto(const Tables& t, const int32_t* who, int requests, int* sums) {
+  const int i = threadIdx.x, lane = threadIdx.x & (kWave - 1);
+  int upto = i < requests ? min(plan_request<FORK>(t, who, i), kSmallPool + 1) : 0;
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int o = __shfl_up(upto, d);
-      if (lane >= d) upto += o;
-    }
-    int total;
-    const int mine = __shfl(upto, kWave - 1);
-    upto += waves_before<kRowWaves>(mine, sums, total) + asked;
-    int fits = i < requests && upto <= free ? upto : 0;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) fits = max(fits, __shfl_xor(fits, d));
-    __syncthreads();
-    if (lane == 0) sums[threadIdx.x / kWave] = fits;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) given = max(given, sums[w]);
-    asked = min(asked + total, kSmallPool + 1);
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int o = __shfl_up(upto, d);
+    if (lane >= d) upto += o;
   }
+  int total;
+  const int mine = __shfl(upto, kWave - 1);
+  return upto + waves_before<kRowWaves>(mine, sums, total);
+}
+
+// Pages given out: the largest sum of leading requests that the free pages suffice for; `upto`: asked_upto.
+__device__ __forceinline__ int given_out(int upto, int free, int* sums) {
+  int fits = upto <= free ? upto : 0;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) fits = max(fits, __shfl_xor(fits, d));
+  __syncthreads();
+  if ((threadIdx.x & (kWave - 1)) == 0) sums[threadIdx.x / kWave] = fits;
+  __syncthreads();
+  int given = 0;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) given = max(given, sums[w]);
   return given;
 }
 
@@ -431,36 +431,22 @@ __global__ __launch_bounds__(kRowWaves* kWave) void fork_small_kernel(Tables t, 
   if (child == children) {
     if (blockIdx.y > 0) return;
     const int free = scan_counts<kRowWaves>(counts, num_blocks, sums, [&](int page, int32_t c, bool, int) { held[page] = max(c, 0); });
-    const int given = given_out<true>(t, parents, children, free, sums);
+    const int upto = asked_upto<true>(t, parents, children, sums);
+    const int given = given_out(upto, free, sums);
     scan_counts<kRowWaves>(counts, num_blocks, sums, [&](int page, int32_t, bool is_free, int rank) {
       if (is_free && rank < given) atomicAdd(held + page, 1);
     });
     // shared pages, of the children whose own page (if they need one) is among those given out
-    int asked = 0;
-    const int lane = threadIdx.x & (kWave - 1);
-    for (int64_t tile = 0; tile < children; tile += kRowWaves * kWave) {
-      const int64_t i = tile + threadIdx.x;
-      const int need = i < children ? plan_request<true>(t, parents, (int)i) : 0;
-      int upto = need;
-#pragma unroll
-      for (int d = 1; d < kWave; d <<= 1) {
-        const int o = __shfl_up(upto, d);
-        if (lane >= d) upto += o;
-      }
-      int total;
-      const int mine = __shfl(upto, kWave - 1);
-      upto += waves_before<kRowWaves>(mine, sums, total) + asked;
-      asked += total;
-      if (i < children) {
-        const int tokens = seq_tokens(t, parents[i]);
-        const bool ok = need == 0 || upto <= free;
-        child_lens[i] = ok ? tokens : 0;
-        if (ok)
-          for (int j = 0; j < tokens / t.block_size; ++j) {
-            const int32_t page = t.tables[(int64_t)parents[i] * t.width + j];
-            if (page >= 0 && page < num_blocks) atomicAdd(held + page, 1);
-          }
-      }
+    const int i = threadIdx.x;
+    if (i < children) {
+      const int tokens = seq_tokens(t, parents[i]);
+      const bool ok = tokens % t.block_size == 0 || upto <= free;
+      child_lens[i] = ok ? tokens : 0;
+      if (ok)
+        for (int j = 0; j < tokens / t.block_size; ++j) {
+          const int32_t page = t.tables[(int64_t)parents[i] * t.width + j];
+          if (page >= 0 && page < num_blocks) atomicAdd(held + page, 1);
+        }
     }
     __syncthreads();
     for (int p = threadIdx.x; p < num_blocks; p += kRowWaves * kWave) new_counts[p] = held[p];
@@ -498,7 +484,7 @@ __global__ __launch_bounds__(kRowWaves* kWave) void extend_small_kernel(Tables t
   const int seq = blockIdx.x;
   if (seq == t.seqs) {
     const int free = scan_counts<kRowWaves>(counts, num_blocks, sums, [](int, int32_t, bool, int) {});
-    const int given = given_out<false>(t, wanted, t.seqs, free, sums);
+    const int given = given_out(asked_upto<false>(t, wanted, t.seqs, sums), free, sums);
     scan_counts<kRowWaves>(counts, num_blocks, sums, [&](int page, int32_t c, bool is_free, int rank) {
       new_counts[page] = is_free ? (rank < given ? 1 : 0) : c;
     });
@@ -625,10 +611,11 @@ static PlanOut plan_layout(void* workspace, int64_t num_blocks) {
   return p;
 }
 
-// Sides of the rule: a beam step of 4 sequences in a pool of 96 pages, three calls: 17.1 us one launch each, 23.0 two
-// each; 128 children in a pool of 1024 pages 80 and 89; the largest of these calls cost as much either way.
+// Sides of the rule (us, one launch and two): a beam step of 4 sequences in a pool of 96 pages, three calls, 17 and 23; 128 children of
+// short sequences in a pool of 4096 pages 9 and 11, 256 in one of 1200 pages 10 and 12, of 4096 pages 14 and 11, 512 17-22 and 14,
+// 2000 91 and 33: every workgroup looks at all requests and all counts.  Extending 256 sequences 8 and 10.
 static bool small_pool(int64_t num_blocks, int64_t requests, int64_t max_pages) {
-  return num_blocks <= kSmallPool && requests <= kSmallEntries && requests * max_pages <= kSmallEntries;
+  return num_blocks <= kSmallPool && requests <= kSmallRequests && requests * max_pages <= kSmallEntries;
 }
 
 static uint32_t page_chunks(int64_t page_elems) { return (uint32_t)((page_elems / 8 + kCopyPieces - 1) / kCopyPieces); }

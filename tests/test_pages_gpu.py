@@ -166,10 +166,10 @@ def test_many_layers_and_pages_larger_than_a_copy_step(paged, dev):
     assert all(_same_bits(a, b) for a, b in zip(caches, want))
 
 
-@pytest.mark.parametrize("requests", [300, 600, 1100])
+@pytest.mark.parametrize("requests", [255, 256, 257, 300, 600, 1100])
 @pytest.mark.parametrize("blocks", [700, 4096])
 def test_more_requests_than_threads(paged, dev, requests, blocks):
-    """One launch up to 16384 table entries, two beyond; pools that run dry in the middle of the requests."""
+    """One launch up to 256 requests, two beyond; pools that run dry in the middle of the requests."""
     block, width = 4, 27
     tables, lens, counts = _pool(requests, blocks, block, 50, width, odd=False)
     r = random.Random(requests)
