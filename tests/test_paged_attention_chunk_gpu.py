@@ -408,3 +408,15 @@ def test_long_tables_at_the_limits_of_the_partition(paged, dev, new, ctx, hq, hk
 def test_tiles_of_every_height(paged, dev, d, window, new, ctx):
     """Around the numbers of rows at which a tile's work is divided differently."""
     _check(paged, dev, _case(new, ctx, 1, 1, d, 16, seed=d), window=window)
+
+
+@pytest.mark.parametrize("d", [16, 144])
+@pytest.mark.parametrize("seqs", [64, 65, 512, 513, 3000, 5000])
+def test_many_sequences(paged, dev, d, seqs):
+    """Sequences without tokens among them, and some of several tiles."""
+    new = [(0, 1, 1, 2, 1, 0, 3)[i % 7] + (300 if i % 1500 == 63 else 0) for i in range(seqs)]
+    _check(paged, dev, _case(new, [n + i % 13 for i, n in enumerate(new)], 1, 1, d, 16, seed=seqs))
+    starts = torch.randint(-50, 900, (seqs + 1,), generator=torch.Generator().manual_seed(1)).int()  # out of order
+    q, kc, vc, tables, ctx, _ = _case([700], [700], 1, 1, d, 16)
+    args = [t.to(dev) for t in (q, kc, vc, tables.expand(seqs, -1).contiguous(), ctx.expand(seqs).contiguous(), starts)]
+    assert paged.paged_attention_chunk(*args, out=torch.zeros_like(args[0])).isfinite().all()
