@@ -375,11 +375,12 @@ __global__ __launch_bounds__(256) void compact_kernel(Tables t, const int32_t* _
 
 // ------------------------------------------------------------------------------------------- small pools
 // The same operators in one launch, for pools of up to kSmallPool pages, up to kSmallRequests requests (one per thread) and
-// tables of up to kSmallEntries entries: a decode step's calls, where each launch counts (about 2 us on the host and as much between two kernels).  Every workgroup finds what it
+// tables of up to kSmallEntries entries, kSmallWalked where one workgroup walks them all: a decode step's calls, where each launch
+// counts (about 2 us on the host and as much between two kernels).  Every workgroup finds what it
 // needs of the plan itself, from counts that are a few KiB in the L2, and one workgroup makes the new counts, in LDS.
 constexpr int kSmallPool = 4096;
 constexpr int kSmallRequests = kRowWaves * kWave;
-constexpr int64_t kSmallEntries = 16384;
+constexpr int64_t kSmallEntries = 16384, kSmallWalked = 4096;
 
 // Pages asked for by the requests in front of request i; called by a workgroup of kRowWaves waves.
 template <bool FORK>
@@ -403,18 +404,49 @@ __device__ __forceinline__ int asked_upto(const Tables& t, const int32_t* who, i
   return upto + waves_before<kRowWaves>(mine, sums, total);
 }
 
+// Largest value of a workgroup of kRowWaves waves; none is negative.
+__device__ __forceinline__ int workgroup_max(int mine, int* sums) {
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) mine = max(mine, __shfl_xor(mine, d));
+  __syncthreads();
+  if ((threadIdx.x & (kWave - 1)) == 0) sums[threadIdx.x / kWave] = mine;
+  __syncthreads();
+  int most = 0;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) most = max(most, sums[w]);
+  return most;
+}
+
 // Pages given out: the largest sum of leading requests that the free pages suffice for; `upto`: asked_upto.
-__device__ __forceinline__ int given_out(int upto, int free, int* sums) {
-  int fits = upto <= free ? upto : 0;
+__device__ __forceinline__ int given_out(int upto, int free, int* sums) { return workgroup_max(upto <= free ? upto : 0, sums); }
+
+// Counts in `held` (LDS) the pages that children share with their parents: the first `full` pages of row `row` for the child
+// that each thread stands for (row 0 where full is 0).  A thread takes (child, page) pairs, eight at a time, whose loads are in
+// flight together: a thread per child, which walks its pages one after the other, took 304 us for one child of 4000 pages and
+// 81 for 1000; so they take 9.2 and 8.2, in two launches, with a workgroup per child, 12.4 and 8.5.
+__device__ __forceinline__ void hold_shared_pages(const Tables& t, int row, int full, int children, int32_t num_blocks, int* rows,
+                                                  int* fulls, int* held, int* sums) {
+  constexpr int kDeep = 8, kThreads = kRowWaves * kWave;
+  rows[threadIdx.x] = row;
+  fulls[threadIdx.x] = full;
+  const int longest = workgroup_max(full, sums);
+  const int pairs = children * longest;
+  const uint32_t inverse = longest > 0 ? 0xffffffffu / longest : 0;  // pair / longest, rounded down: at most one too small
+  for (int first = threadIdx.x; first < pairs; first += kThreads * kDeep) {
+    int32_t page[kDeep];
+    bool is[kDeep];
 #pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) fits = max(fits, __shfl_xor(fits, d));
-  __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) sums[threadIdx.x / kWave] = fits;
-  __syncthreads();
-  int given = 0;
+    for (int k = 0; k < kDeep; ++k) {
+      const int pair = min(first + k * kThreads, pairs - 1);
+      int child = __umulhi(pair, inverse), j = pair - child * longest;
+      if (j >= longest) ++child, j -= longest;
+      is[k] = first + k * kThreads < pairs && j < fulls[child];
+      page[k] = t.tables[(int64_t)rows[child] * t.width + j];
+    }
 #pragma unroll
-  for (int w = 0; w < kRowWaves; ++w) given = max(given, sums[w]);
-  return given;
+    for (int k = 0; k < kDeep; ++k)
+      if (is[k] && page[k] >= 0 && page[k] < num_blocks) atomicAdd(held + page[k], 1);
+  }
 }
 
 // Workgroup (child, y) as in fork_kernel; workgroup (children, 0) makes the counts and lengths.
@@ -427,6 +459,7 @@ __global__ __launch_bounds__(kRowWaves* kWave) void fork_small_kernel(Tables t, 
   __shared__ int sums[kRowWaves];
   __shared__ int fresh;
   __shared__ int held[kSmallPool];
+  __shared__ int rows[kSmallRequests], fulls[kSmallRequests];
   const int child = blockIdx.x;
   if (child == children) {
     if (blockIdx.y > 0) return;
@@ -438,16 +471,14 @@ __global__ __launch_bounds__(kRowWaves* kWave) void fork_small_kernel(Tables t, 
     });
     // shared pages, of the children whose own page (if they need one) is among those given out
     const int i = threadIdx.x;
+    int full = 0;
     if (i < children) {
       const int tokens = seq_tokens(t, parents[i]);
       const bool ok = tokens % t.block_size == 0 || upto <= free;
       child_lens[i] = ok ? tokens : 0;
-      if (ok)
-        for (int j = 0; j < tokens / t.block_size; ++j) {
-          const int32_t page = t.tables[(int64_t)parents[i] * t.width + j];
-          if (page >= 0 && page < num_blocks) atomicAdd(held + page, 1);
-        }
+      if (ok) full = tokens / t.block_size;
     }
+    hold_shared_pages(t, full > 0 ? parents[i] : 0, full, children, num_blocks, rows, fulls, held, sums);
     __syncthreads();
     for (int p = threadIdx.x; p < num_blocks; p += kRowWaves * kWave) new_counts[p] = held[p];
     return;
@@ -614,8 +645,11 @@ static PlanOut plan_layout(void* workspace, int64_t num_blocks) {
 // Sides of the rule (us, one launch and two): a beam step of 4 sequences in a pool of 96 pages, three calls, 17 and 23; 128 children of
 // short sequences in a pool of 4096 pages 9 and 11, 256 in one of 1200 pages 10 and 12, of 4096 pages 14 and 11, 512 17-22 and 14,
 // 2000 91 and 33: every workgroup looks at all requests and all counts.  Extending 256 sequences 8 and 10.
-static bool small_pool(int64_t num_blocks, int64_t requests, int64_t max_pages) {
-  return num_blocks <= kSmallPool && requests <= kSmallRequests && requests * max_pages <= kSmallEntries;
+// `most` entries of the requests' rows: the pages of forks and of sequences that end are counted by one workgroup, 4000 of them in 9.2
+// and 9.2-12.0 (fork), 5.0 and 6.5-10.1 (free), 16000 in 15.7 and 9.3, 11.6 and 6.6; rows are extended by a workgroup each, 16000
+// entries in 7.9-9.9 and 8.2-8.5.
+static bool small_pool(int64_t num_blocks, int64_t requests, int64_t max_pages, int64_t most) {
+  return num_blocks <= kSmallPool && requests <= kSmallRequests && requests * max_pages <= most;
 }
 
 static uint32_t page_chunks(int64_t page_elems) { return (uint32_t)((page_elems / 8 + kCopyPieces - 1) / kCopyPieces); }
@@ -665,7 +699,7 @@ extern "C" int aops_fork_sequences_f16(const int32_t* block_tables, const int32_
   const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
   // a slice is at most four rounds of a workgroup's copy loop, unless a page is larger than 64 of them
   const uint32_t slices = (uint32_t)std::min<int64_t>((row_elems * block_size / 8 + 4 * kCopyPieces - 1) / (4 * kCopyPieces), 64);
-  if (small_pool(num_blocks, children, max_pages)) {
+  if (small_pool(num_blocks, children, max_pages, kSmallWalked)) {
     fork_small_kernel<<<dim3((unsigned)children + 1, 1 + (unsigned)num_caches * slices), kRowWaves * kWave, 0, st>>>(
         t, parents, (int32_t)children, c, slices, ref_counts, (int32_t)num_blocks, (uint32_t)(row_elems / 16), child_tables,
         child_lens, new_ref_counts);
@@ -696,7 +730,7 @@ extern "C" int aops_extend_sequences(const int32_t* block_tables, const int32_t*
   if (!workspace || workspace_bytes < aops_pages_workspace(seqs, num_blocks)) return AOPS_ERR_WORKSPACE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
-  if (small_pool(num_blocks, seqs, max_pages)) {
+  if (small_pool(num_blocks, seqs, max_pages, kSmallEntries)) {
     extend_small_kernel<<<(unsigned)seqs + 1, kRowWaves * kWave, 0, st>>>(t, wanted_lens, ref_counts, (int32_t)num_blocks,
                                                                            new_tables, granted_lens, new_ref_counts);
     return record_launch_status(hipGetLastError());
@@ -722,7 +756,7 @@ extern "C" int aops_free_sequences(const int32_t* block_tables, const int32_t* c
     return AOPS_ERR_INVALID_ARGUMENT;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Tables t = {block_tables, context_lens, (int32_t)seqs, (int32_t)max_pages, (int32_t)block_size};
-  if (small_pool(num_blocks, seqs > 0 ? num_rows : 0, max_pages)) {
+  if (small_pool(num_blocks, seqs > 0 ? num_rows : 0, max_pages, kSmallWalked)) {
     free_small_kernel<<<1, kPlanWaves * kWave, 0, st>>>(t, rows, (int32_t)(seqs > 0 ? num_rows : 0), ref_counts,
                                                         (int32_t)num_blocks, new_ref_counts);
     return record_launch_status(hipGetLastError());

@@ -261,3 +261,67 @@ def test_two_streams_at_once(paged, dev, blocks):
                 got[i].append(step(i))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g, w in zip(got, want) for x in g for a, b in zip(x, w))
+
+
+@pytest.mark.parametrize("blocks,children,pages", [(4096, 1, 4000), (4096, 1, 1000), (4096, 4, 1000), (4096, 16, 250), (4000, 7, 580), (4096, 256, 11),
+                                                   (4096, 4, 4000), (4096, 16, 1000), (4096, 256, 60)])
+def test_children_of_long_parents_in_a_small_pool(paged, dev, blocks, children, pages):
+    """Shared pages are counted by (child, page): children of one parent and of several, refused ones and parents that
+    are none among them, more pairs than a workgroup looks at in one round."""
+    block, seqs = 16, max(1, min(3, blocks // pages))
+    width = pages + 5
+    r = random.Random(pages + children)
+    order = r.sample(range(blocks), pages * seqs)
+    tables = [order[b * pages:(b + 1) * pages] + [-1] * (width - pages) for b in range(seqs)]
+    lens = [pages * block - (0, 5, block - 1)[b] for b in range(seqs)]
+    counts = [0] * blocks
+    for p in order:
+        counts[p] += 1
+    for free in (2, blocks):  # all but two of the free pages are given away first: some children get none
+        kept = 0
+        for p in range(blocks):
+            if counts[p] == 0:
+                kept += 1
+                counts[p] = 0 if kept <= free else 1
+        parents = [r.randrange(-1, seqs + 1) if children > 1 else seqs - 1 for _ in range(children)]
+        ref = S.PoolRef(counts, block)
+        rows, out = ref.fork(tables, lens, parents)
+        caches = _caches(dev, blocks, 16, block, 1)
+        want = [ref.moved(x.cpu()) for x in caches]
+        t, l, p, c = _dev(dev, tables, lens, parents, counts)
+        got = paged.fork_sequences(t, l, p, c, caches[:1], caches[1:])
+        assert got[0].tolist() == rows and got[1].tolist() == out and got[2].tolist() == ref.counts
+        assert all(_same_bits(a, b) for a, b in zip(caches, want))
+
+
+def _microseconds(f, calls=20, rounds=7):
+    """Median over rounds of the time of a call among others."""
+    f()
+    times = []
+    for _ in range(rounds):
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        begin.record()
+        for _ in range(calls):
+            f()
+        end.record()
+        end.synchronize()
+        times.append(begin.elapsed_time(end) * 1000 / calls)
+    return sorted(times)[rounds // 2]
+
+
+@pytest.mark.parametrize("op", ["fork", "free"])
+@pytest.mark.parametrize("rows,pages", [(1, 4000), (4, 1000), (16, 1000)])
+def test_one_launch_is_not_far_slower_than_two(paged, dev, op, rows, pages):
+    """Long sequences cost about the same on both sides of the largest pool that takes one launch (a fork 25 times as
+    much where one thread walked all pages of a child)."""
+    us = []
+    for blocks in (4096, 4097):
+        caches = _caches(dev, blocks, 16, 16, 1)
+        tables = [[j for j in range(pages)] + [-1] * 8]
+        counts = [1] * pages + [0] * (blocks - pages)
+        t, l, p, c = _dev(dev, tables, [pages * 16 - 5], [0] * rows, counts)
+        if op == "fork":
+            us.append(_microseconds(lambda: paged.fork_sequences(t, l, p, c, caches[:1], caches[1:])))
+        else:
+            us.append(_microseconds(lambda: paged.free_sequences(t, l, p, c, 16)))
+    assert us[0] < 4 * us[1], us
