@@ -112,3 +112,27 @@ def test_tile_kernels_keep_their_registers(assembly):
     for name in CHUNK:
         sizes = re.findall(r"\.amdhsa_kernel _ZN4aops\d+chunk_tiles_kernel\w+\n.*?private_segment_fixed_size (\d+)", assembly[name], re.S)
         assert len(sizes) == 2 and set(sizes) == {"0"}, name
+
+
+def _loads_together(lines):
+    """Numbers of memory loads that are issued without a wait for one, or a branch, between them."""
+    found, run = [], 0
+    for line in lines + ["s_branch"]:
+        if re.match(r"global_load_(?!lds)", line):
+            run += 1
+        elif "vmcnt" in line or line.startswith(("s_branch", "s_cbranch")):
+            found += [run] if run else []
+            run = 0
+    return found
+
+
+def test_counts_of_pages_are_loaded_together(assembly):
+    """A lane's eight counts of a pass over the pool are on their way at once, in every kernel that makes such passes."""
+    passes = {"compact_plan_kernel": 2, "fork_small_kernel": 3, "extend_small_kernel": 4, "compact_small_kernel": 2, "pages_plan_kernel": 1}
+    seen = dict.fromkeys(passes, 0)
+    for m in re.finditer(r"^_ZN4aops\d+(\w+?_kernel)\w*:[^\n]*\n(.*?)^\.Lfunc_end", assembly["pages.hip"], re.S | re.M):
+        if m.group(1) in passes:
+            seen[m.group(1)] += 1
+            lines = [line.split(";")[0].strip() for line in m.group(2).split("\n")]
+            assert sum(n == 8 for n in _loads_together(lines)) >= passes[m.group(1)], m.group(1)
+    assert seen == {**dict.fromkeys(passes, 1), "pages_plan_kernel": 2}, seen
