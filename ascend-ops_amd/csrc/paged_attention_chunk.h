@@ -97,9 +97,14 @@ struct ChunkTile {
   int unit0, units;     // in units of kChunkUnit tokens, at least one
 };
 
+// First row and number of rows between two bounds.
+__device__ __forceinline__ void chunk_rows_between(ChunkArgsRef a, int start, int end, int& q0, int& n) {
+  q0 = min(max(start, 0), a.tokens);
+  n = min(max(end, q0), a.tokens) - q0;
+}
+
 __device__ __forceinline__ void chunk_seq(ChunkArgsRef a, int b, int& q0, int& n) {
-  q0 = min(max(a.query_starts[b], 0), a.tokens);
-  n = min(max(a.query_starts[b + 1], q0), a.tokens) - q0;
+  chunk_rows_between(a, a.query_starts[b], a.query_starts[b + 1], q0, n);
 }
 
 __device__ __forceinline__ int chunk_tiles(ChunkArgsRef a, int n) {
@@ -925,14 +930,20 @@ __device__ __forceinline__ bool chunk_find(ChunkArgsRef a, int tile, int* shared
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const bool alone = a.seqs <= PER * kWave;
   int running = 0;  // tiles of the sequences in front
-  for (int64_t base = 0; base < a.seqs; base += PER * kWave * WAVES) {
-    const int64_t first = base + (int64_t)(alone ? lane : threadIdx.x) * PER;
-    int tiles[PER], mine = 0;
+  for (uint32_t base = 0; base < (uint32_t)a.seqs; base += PER * kWave * WAVES) {
+    const uint32_t own = base + (alone ? lane : threadIdx.x) * PER, first = min(own, (uint32_t)(a.seqs - PER));
+    // A lane's bounds lie next to each other and are on their way at once (a pair for each sequence, under a condition of its own, was
+    // waited for: 512 decoding sequences 169 us instead of 164, 8000 2.74 ms instead of 2.66).  The last lanes with sequences read the last PER and leave out those in front of their own.
+    int bounds[PER + 1], tiles[PER], mine = 0;
+#pragma unroll
+    for (int i = 0; i <= PER; ++i) bounds[i] = a.query_starts[first + i];
+#pragma unroll
+    for (int i = 0; i <= PER; ++i) asm volatile("" : "+v"(bounds[i]));  // (else the compiler moves the first load into a branch)
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      int q0, n = 0;
-      if (first + i < a.seqs) chunk_seq(a, (int)(first + i), q0, n);
-      tiles[i] = chunk_tiles(a, n);
+      int q0, n;
+      chunk_rows_between(a, bounds[i], bounds[i + 1], q0, n);
+      tiles[i] = first + i >= own ? chunk_tiles(a, n) : 0;
       mine += tiles[i];
     }
     mine = min(mine, a.max_tiles);  // (bounds that overlap count tokens again and again: what is behind max_tiles is not looked for)

@@ -136,3 +136,23 @@ def test_counts_of_pages_are_loaded_together(assembly):
             lines = [line.split(";")[0].strip() for line in m.group(2).split("\n")]
             assert sum(n == 8 for n in _loads_together(lines)) >= passes[m.group(1)], m.group(1)
     assert seen == {**dict.fromkeys(passes, 1), "pages_plan_kernel": 2}, seen
+
+
+def test_bounds_of_sequences_are_loaded_together(assembly):
+    """A lane that looks for a tile among eight sequences has their nine bounds on their way at once."""
+    seen = 0
+    for name in CHUNK:
+        for kind, d, lines in _chunk_kernels(assembly[name]):
+            if kind != "tiles":
+                continue
+            found, dwords = set(), 0
+            for line in lines:
+                load = re.match(r"global_load_dword(?:x(\d))? ", line)
+                if load:
+                    dwords += int(load.group(1) or 1)
+                elif "vmcnt" in line or line.startswith(("s_branch", "s_cbranch")):
+                    found.add(dwords)
+                    dwords = 0
+            assert 9 in found, (d, found)
+            seen += 1
+    assert seen == 16
