@@ -635,8 +635,9 @@ static bool geometry_ok(int64_t num_caches, int64_t num_blocks, int64_t row_elem
          row_elems * block_size / 8 <= 0x7fffffff;  // 16-byte pieces of a page are counted in 32 bits
 }
 
+// (A workgroup counts the columns of a row in 32 bits, 256 at a time: behind 2^31 - 256 of them the last step would wrap.)
 static bool tables_ok(int64_t seqs, int64_t max_pages, int64_t block_size) {
-  return seqs >= 0 && seqs <= 0x7fffffff && max_pages >= 0 && max_pages <= 0x7fffffff && block_size > 0 &&
+  return seqs >= 0 && seqs <= 0x7fffffff && max_pages >= 0 && max_pages <= 0x7fffff00 && block_size > 0 &&
          block_size <= 0x7fffffff;
 }
 

@@ -195,7 +195,7 @@ int aops_rotary_f16(const void* q, const void* k, const int32_t* position_ids, c
  * Pages of the paged caches.  `caches`: HOST array of num_caches (1 to 256) device pointers, the key and value caches
  * of all layers, each [num_blocks, row_elems/16, block_size, 16]; it is read during the call only.  ref_counts: int32
  * [num_blocks] on the device, the number of sequences that hold a page; a page is free where it is not positive.
- * block_tables: int32 [seqs, max_pages], context_lens: int32 [seqs]; a sequence holds the first
+ * block_tables: int32 [seqs, max_pages], max_pages up to 2^31 - 256, context_lens: int32 [seqs]; a sequence holds the first
  * ceil(context_len / block_size) entries of its row (lengths are limited to 0 .. max_pages * block_size).  Tables and
  * counts are read, new ones are written to other memory; negative counts come out as 0.  Table entries and page
  * numbers outside the caches are passed on, and neither counted nor copied.  Pages are given out lowest first, in the

@@ -202,3 +202,15 @@ def test_c_abi_chunk_attention():
     assert size(100000, 1, 2, 1, 128, 1 << 16, 32767) == 16  # the partition counts in 32 bits
     assert run(pages=400, ws_bytes=size(4, 2, 4, 2, 64, 16, 400) - 1) == -2
     assert size(4, 2, 5, 2, 64, 16, 4) == 0 and size(4, 2, 4, 2, 24, 16, 4) == 0
+
+
+def test_c_abi_pages_refuse_rows_that_pass_32_bits():
+    """A workgroup counts the columns of a row in 32 bits, in steps of its threads: the last step must not wrap."""
+    lib = cabi.lib()
+    p = ctypes.c_void_p(16)
+    many = (ctypes.c_void_p * 2)(16, 16)
+    for width in (0x7fffff01, 0x7fffffff):
+        assert lib.aops_fork_sequences_f16(p, p, 1, width, p, 1, p, 8, many, 2, 64, 16, p, p, p, p, 1 << 20, None) == -1
+        assert lib.aops_extend_sequences(p, p, p, 1, width, 16, p, 8, p, p, p, p, 1 << 20, None) == -1
+        assert lib.aops_free_sequences(p, p, 1, width, 16, p, 1, p, 8, p, None) == -1
+        assert lib.aops_compact_pages_f16(p, p, 1, width, p, 8, many, 2, 64, 16, p, p, p, p, 1 << 20, None) == -1
