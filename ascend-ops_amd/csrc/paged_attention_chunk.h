@@ -62,6 +62,7 @@ constexpr float kChunkNegBig = -1.0e30f;
 constexpr float kChunkLog2e = 1.4426950408889634f;
 constexpr float kChunkLn2 = 0.6931471805599453f;
 constexpr float kChunkLift = 6.0f, kChunkSlack = 8.0f;
+constexpr float kChunkFar = 1024.0f;  // up to here kChunkLift - ref is off by 2^-14 at most, a weight by an eighth of its rounding to fp16
 
 struct ChunkArgs {
   const f16 *q, *key_cache, *value_cache;
@@ -260,6 +261,7 @@ struct ChunkState {
   f32x4 o[CB][ChunkDims<D>::kBlocks];  // O^T: lane (row n, kg), element i <-> d = 16 block + 4kg + i
   float ref[CB];                       // reference value of the row's weights, log2 units
   float sum[CB];                       // this lane's share of the sum of weights
+  uint64_t far;                        // not 0: a row of the wave has its reference value far from zero
 };
 
 template <int D, int CB>
@@ -298,6 +300,7 @@ __device__ __forceinline__ void chunk_init(ChunkState<D, CB>& st) {
     st.ref[c] = kChunkNegBig;
     st.sum[c] = 0.f;
   }
+  st.far = 0;
 }
 
 // Scores out of sight become -inf.  Lane (row n, kg) has tokens token0 + 16g + 4kg + i.
@@ -366,15 +369,36 @@ __device__ __forceinline__ void chunk_softmax(f32x4 (&s)[CB][KG], float scale, C
 #pragma unroll
         for (int i = 0; i < 4; ++i) st.o[c][db][i] *= alpha;
     }
+    bool far = false;
+#pragma unroll
+    for (int c = 0; c < CB; ++c) far |= __builtin_fabsf(st.ref[c]) > kChunkFar && st.ref[c] > kChunkNegBig;
+    st.far = __builtin_amdgcn_ballot_w64(far);
+  }
+  // A weight is exp2(s scale + (kChunkLift - ref)), with one rounding of the bracket and one of the sum: where the reference value is
+  // so large that these are not small, the score is rounded first, as the reference value was, so that the largest one's distance
+  // from it is what it is, down to 0 (else scores of 2^25 and more left infinite weights, or none).
+  float base[CB];
+#pragma unroll
+  for (int c = 0; c < CB; ++c) base[c] = kChunkLift - st.ref[c];
+  if (__builtin_expect(st.far != 0, 0)) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      base[c] = kChunkLift;
+#pragma unroll
+      for (int g = 0; g < KG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[c][g][i] = s[c][g][i] * scale - st.ref[c];
+    }
+    scale = 1.0f;
   }
 #pragma unroll
   for (int c = 0; c < CB; ++c) {
-    const float base = kChunkLift - st.ref[c];
     float sum[KG];
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[c][g][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][g][i], scale, base));
+      for (int i = 0; i < 4; ++i) s[c][g][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][g][i], scale, base[c]));
       sum[g] = (s[c][g][0] + s[c][g][1]) + (s[c][g][2] + s[c][g][3]);
     }
     float all = KG == 4 ? (sum[0] + sum[1]) + (sum[KG - 2] + sum[KG - 1]) : sum[0] + sum[1];

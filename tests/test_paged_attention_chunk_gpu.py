@@ -420,3 +420,36 @@ def test_many_sequences(paged, dev, d, seqs):
     q, kc, vc, tables, ctx, _ = _case([700], [700], 1, 1, d, 16)
     args = [t.to(dev) for t in (q, kc, vc, tables.expand(seqs, -1).contiguous(), ctx.expand(seqs).contiguous(), starts)]
     assert paged.paged_attention_chunk(*args, out=torch.zeros_like(args[0])).isfinite().all()
+
+
+@pytest.mark.parametrize("new,ctx", [([3, 1], [700, 40]), ([60, 1], [300, 9]), ([300], [2900]), ([4], [4000])])
+@pytest.mark.parametrize("d", [64, 128, 208])
+@pytest.mark.parametrize("size,scale", [(1000.0, None), (60000.0, None), (60000.0, 2.0 ** 56), (0.5, 2.0 ** 56), (2.0, 2.0 ** 20)])
+def test_scores_far_from_zero(paged, dev, new, ctx, d, size, scale):
+    """Queries and keys as large as fp16 goes, and large scales: keys that are all alike weigh the same, however large their
+    score, and keys whose score is far above the others' are all that counts.
+
+    All elements of a query are one number, all of a key that number times a power of two (or cut off), so equal keys have
+    equal scores in any arithmetic and the others' are far below.  Rounded are the score (a sum of D products, half a step each, and
+    its scaling), the weights, which are all the same, once to fp16, the sums (half a step per 32 keys, and 16 for joins) and the result."""
+    block = 16
+    q, kc, vc, tables, lens, starts = _case(new, ctx, 4, 2, d, block, seed=d)
+    q, tables, vc = torch.full_like(q, size), tables.clamp(max=kc.shape[0] - 1), vc.nan_to_num(0, 0, 0)
+    for sign in (1, -1):
+        for levels in (1, 6):
+            level = torch.zeros(kc.shape[0], block)
+            for b, n in enumerate(ctx):  # the maximum comes early, or late, or again and again
+                for tok in range(n):
+                    level[tables[b, tok // block].long(), tok % block] = tok * 7 % 11 % levels
+            k = (sign * size * 2.0 ** -(level if sign < 0 else 5 - level)).clamp(-60000, 60000).half()
+            kc = k[:, None, :, None].expand(-1, kc.shape[1], -1, 16).contiguous()
+            want, want_lse = S.paged_attention_chunk_ref(q, kc, vc, tables, lens, starts, scale=scale)
+            o, lse = paged.paged_attention_chunk(*(t.to(dev) for t in (q, kc, vc, tables, lens, starts)), scale=scale, return_lse=True)
+            o, lse = o.cpu().double(), lse.cpu().double()
+            finite, what = bool(o.isfinite().all() and lse.isfinite().all()), (sign, levels)
+            assert finite, what
+            worst = float(((lse - want_lse).abs() - want_lse.abs() * 2.0 ** -24 * (d + 4)).max())
+            assert worst <= 2.0 ** -18, (what, worst)
+            tol = want.abs() * 2.0 ** -10 + (max(ctx) / 32 + 16) * 2.0 ** -24 * float(vc.abs().max()) + 2.0 ** -24
+            worst = float(((o - want).abs() / tol).max())
+            assert worst <= 1, (what, worst)
