@@ -498,7 +498,7 @@ py::object paged_attention_chunk(const Tensor& q, const Tensor& key_cache, const
   TORCH_CHECK(query_starts.size(0) == seqs + 1, name, ": query_starts must have one entry more than block_tables has rows, got ",
               query_starts.size(0), " and ", seqs);
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)head_dim);
-  TORCH_CHECK(std::isfinite((float)s) && (float)s > 0.f, name, ": scale must be positive and finite, got ", s);
+  TORCH_CHECK((float)s > 0.f && (float)s <= 0x1p56f, name, ": scale must be positive and at most 2^56, got ", s);
   TORCH_CHECK(window >= 0, name, ": window must not be negative, got ", window);
   require_device(name, {{"q", q, at::kHalf},
                         {"key_cache", key_cache, at::kHalf},

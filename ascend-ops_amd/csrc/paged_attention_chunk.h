@@ -59,6 +59,7 @@ constexpr int kChunkWorth = 8;     // what cutting tiles costs, in units
 constexpr int kChunkPlanHead = 4;  // ints in front of the plan: units per share
 constexpr int kChunkMaxTiles = 1024;  // of the balanced partition
 constexpr float kChunkNegBig = -1.0e30f;
+constexpr float kChunkMaxScale = 0x1p56f;  // a score of up to 256 elements of fp16 (below 2^40) then stays above kChunkNegBig
 constexpr float kChunkLog2e = 1.4426950408889634f;
 constexpr float kChunkLn2 = 0.6931471805599453f;
 constexpr float kChunkLift = 6.0f, kChunkSlack = 8.0f;

@@ -1,7 +1,5 @@
 // Entry points of the attention of a chunk of new tokens per sequence over the paged caches, the choice between the two
 // partitions of its work, and the kernel that joins partial results.  The kernels proper: paged_attention_chunk.h.
-#include <math.h>
-
 #include <algorithm>
 
 #include "paged_attention_chunk.h"
@@ -110,7 +108,7 @@ extern "C" int aops_paged_attention_chunk_f16(const void* q, const void* key_cac
                                               int64_t max_pages, int64_t num_blocks, void* stream) {
   using namespace aops;
   if (!chunk_sizes_ok(tokens, seqs, num_heads, num_kv_heads, head_dim, block_size, max_pages) || num_blocks < 0 ||
-      num_blocks > 0x7fffffff || window < 0 || !(scale > 0.f) || !isfinite(scale))
+      num_blocks > 0x7fffffff || window < 0 || !(scale > 0.f) || !(scale <= kChunkMaxScale))
     return AOPS_ERR_INVALID_ARGUMENT;
   if (tokens == 0 || seqs == 0) return AOPS_OK;
   if (!q || !out || !context_lens || !query_starts) return AOPS_ERR_INVALID_ARGUMENT;

@@ -137,7 +137,7 @@ int aops_qknorm_rope_reshape_and_cache_f16(
  * key_cache, value_cache: [num_blocks, num_kv_heads*head_dim/16, block_size, 16]; block_tables: int32 [seqs, max_pages]
  * (entries outside the cache read the nearest page; keys that no entry of the row holds do not exist); context_lens: int32
  * [seqs]; query_starts: int32 [seqs + 1], not decreasing (bounds are limited to 0 .. tokens).  lse: fp32
- * [tokens, num_heads] or NULL.  scale is positive and finite.  What lies in the cache where a row does not see it, infinities
+ * [tokens, num_heads] or NULL.  scale is positive and at most 2^56.  What lies in the cache where a row does not see it, infinities
  * and NaN included, has no effect on it.
  * head_dim: a multiple of 16 up to 256; num_heads a multiple of num_kv_heads; tokens * num_heads / num_kv_heads below 2^30.
  * workspace: aops_paged_attention_chunk_workspace bytes (queried with the same device current; 0 = unsupported shape), not

@@ -214,3 +214,14 @@ def test_c_abi_pages_refuse_rows_that_pass_32_bits():
         assert lib.aops_extend_sequences(p, p, p, 1, width, 16, p, 8, p, p, p, p, 1 << 20, None) == -1
         assert lib.aops_free_sequences(p, p, 1, width, 16, p, 1, p, 8, p, None) == -1
         assert lib.aops_compact_pages_f16(p, p, 1, width, p, 8, many, 2, 64, 16, p, p, p, p, 1 << 20, None) == -1
+
+
+def test_chunk_attention_refuses_scales_that_leave_fp32():
+    """With 2^56 the scores of any finite queries and keys can be told from a masked place; beyond that rows could come out
+    as if they saw nothing."""
+    from ascend910a_extras.paged import paged_attention_chunk as f
+
+    lib, p = cabi.lib(), ctypes.c_void_p(16)
+    for scale in (2.0 ** 57, 1e27, 3e38):
+        assert lib.aops_paged_attention_chunk_f16(p, p, p, p, p, p, p, None, scale, 0, p, 1 << 30, 4, 2, 4, 2, 64, 16, 4, 8, None) == -1
+        _raises(f, _half(3, 4, 64), _half(8, 8, 16, 16), _half(8, 8, 16, 16), _int(2, 4), _int(2), _int(3), scale=scale, match="2\\^56")
