@@ -69,7 +69,8 @@ def extend_sequences(block_tables: Tensor, context_lens: Tensor, wanted_lens: Te
                      block_size: int) -> tuple[Tensor, Tensor, Tensor]:
     """Pages for ``wanted_lens`` (int32 ``[sequences]``) tokens.  Returns ``(new_tables, granted_lens, new_ref_counts)``: where a
     row of the table is too short, or the free pages do not suffice for a sequence and all those in front of it, its
-    row and length stay as they are; lengths never shrink."""
+    row and length stay as they are, and likewise where the length wanted is not greater than the present one.  A present length
+    that its row cannot hold counts, and comes back, as what the row holds, a negative one as 0."""
     return _C.extend_sequences(block_tables, context_lens, wanted_lens, ref_counts, block_size)
 
 

@@ -325,3 +325,15 @@ def test_one_launch_is_not_far_slower_than_two(paged, dev, op, rows, pages):
         else:
             us.append(_microseconds(lambda: paged.free_sequences(t, l, p, c, 16)))
     assert us[0] < 4 * us[1], us
+
+
+@pytest.mark.parametrize("blocks", [60, 5000])
+def test_lengths_outside_their_rows_come_back_limited(paged, dev, blocks):
+    """A present length counts as far as the row can hold it, from 0 on; whatever is wanted, the row is full or empty."""
+    block, width = 16, 4
+    t, l, w, c = _dev(dev, [[0, 1, 2, 3], [4, 5, 6, 7], [-1] * 4, [-1] * 4, [8, 9, -1, -1]], [64 + 9, 2 ** 31 - 1, -3, -2 ** 31, 20],
+                      [80, 10, 17, 0, 5], [1] * 10 + [0] * (blocks - 10))
+    tables, lens, counts = paged.extend_sequences(t, l, w, c, block)
+    assert lens.tolist() == [64, 64, 17, 0, 20]
+    assert tables.tolist() == [[0, 1, 2, 3], [4, 5, 6, 7], [10, 11, -1, -1], [-1] * 4, [8, 9, -1, -1]]
+    assert counts.tolist() == [1] * 12 + [0] * (blocks - 12)
