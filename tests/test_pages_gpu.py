@@ -337,3 +337,45 @@ def test_lengths_outside_their_rows_come_back_limited(paged, dev, blocks):
     assert lens.tolist() == [64, 64, 17, 0, 20]
     assert tables.tolist() == [[0, 1, 2, 3], [4, 5, 6, 7], [10, 11, -1, -1], [-1] * 4, [8, 9, -1, -1]]
     assert counts.tolist() == [1] * 12 + [0] * (blocks - 12)
+
+
+def test_pages_beyond_four_gigabytes(paged, dev):
+    """Offsets that pass 32 bits, in bytes and in elements: copies, a fork and packing at the far end of a cache of 9 GiB."""
+    row, block = 1024, 128
+    blocks = (9 << 30) // (row * block * 2)  # 36864 pages of 256 KiB
+    kc = torch.zeros(blocks, row // 16, block, 16, dtype=H, device=dev)
+    vc = torch.zeros_like(kc)
+    g = torch.Generator().manual_seed(8)
+
+    def fill(*pages):
+        for p in pages:
+            for c in (kc, vc):
+                c[p] = torch.randint(-32768, 32768, c.shape[1:], generator=g, dtype=torch.int16).view(H).to(dev)
+
+    far, middle = blocks - 1, blocks - 2 - (4 << 30) // (row * block * 2)
+    fill(far, 3)
+    s, d = _dev(dev, [far, 3], [middle, far - 1])
+    paged.copy_pages([kc], [vc], s, d)
+    for c in (kc, vc):
+        assert _same_bits(c[middle], c[far]) and _same_bits(c[far - 1], c[3]) and not c[far - 2].any() and not c[0].any()
+    # a child of a parent whose last page is the far one, into the only free pages, both far out too
+    counts = torch.ones(blocks, dtype=I, device=dev)
+    counts[far - 1] = counts[far - 2] = 0
+    kc[far - 1], vc[far - 1] = 0, 0
+    t, l, p = _dev(dev, [[middle, far]], [block + 77], [0, 0])
+    rows, lens, after = paged.fork_sequences(t, l, p, counts, [kc], [vc])
+    assert rows.tolist() == [[middle, far - 2], [middle, far - 1]] and lens.tolist() == [block + 77] * 2
+    assert after[middle] == 3 and after[far - 1] == after[far - 2] == 1
+    for c in (kc, vc):
+        for page in (far - 2, far - 1):
+            assert _same_bits(c[page, :, :77], c[far, :, :77]) and not c[page, :, 77:].any()
+    # the far pages to the lowest ones
+    counts.zero_()
+    counts[far], counts[middle], counts[1] = 1, 2, 1
+    want = [(c[middle].clone(), c[far].clone()) for c in (kc, vc)]
+    kept = kc[1].clone()
+    rows, after, used = paged.compact_pages(*_dev(dev, [[middle, far], [1, middle]], [block + 77, block + 1]), counts, [kc], [vc])
+    assert rows.tolist() == [[0, 2], [1, 0]] and used.item() == 3 and after[:4].tolist() == [2, 1, 1, 0] and not after[4:].any()
+    for c, (first, second) in zip((kc, vc), want):
+        assert _same_bits(c[0], first) and _same_bits(c[2], second)
+    assert _same_bits(kc[1], kept)
