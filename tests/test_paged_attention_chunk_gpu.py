@@ -453,3 +453,80 @@ def test_scores_far_from_zero(paged, dev, new, ctx, d, size, scale):
             tol = want.abs() * 2.0 ** -10 + (max(ctx) / 32 + 16) * 2.0 ** -24 * float(vc.abs().max()) + 2.0 ** -24
             worst = float(((o - want).abs() / tol).max())
             assert worst <= 1, (what, worst)
+
+
+def _check_bounds(paged, dev, case, starts):
+    """Limited bounds, sequence by sequence: rows of exactly one sequence against the definition, rows of none untouched (rows of
+    several are one of theirs, or a mixture).  How many rows there are of each kind."""
+    q, kc, vc, tables, ctx, _ = case
+    rows = q.shape[0]
+    want = torch.full(q.shape, math.nan, dtype=torch.float64)
+    times = torch.zeros(rows, dtype=torch.long)
+    for b in range(len(ctx)):
+        begin = min(max(int(starts[b]), 0), rows)
+        end = min(max(int(starts[b + 1]), begin), rows)
+        if begin == end:
+            continue
+        own = torch.tensor([0, end - begin], dtype=I)
+        want[begin:end] = S.paged_attention_chunk_ref(q[begin:end], kc, vc, tables[b:b + 1], ctx[b:b + 1], own)[0]
+        times[begin:end] += 1
+    out = torch.full_like(q, 7.0).to(dev)
+    got = paged.paged_attention_chunk(*(t.to(dev) for t in (q, kc, vc, tables, ctx, starts)), out=out).cpu().double()
+    assert (got[times == 0] == 7).all()
+    once = times == 1
+    tol, _ = _tolerances((q, kc, vc, tables, ctx, starts), None, None, q.shape[-1] ** -0.5, 0, (want[once], torch.zeros(1)))
+    assert ((got[once] - want[once]).abs() <= tol).all(), float(((got[once] - want[once]).abs() / tol).max())
+    return [int((times == n).sum()) for n in (0, 1)]
+
+
+@pytest.mark.parametrize("starts,untouched,once", [([-9, 4, 54, 99], 0, 57), ([0, 4, 54, 57], 0, 57), ([3, 4, 50, 50], 10, 47), ([0, 4, 2, 57], 0, 55),
+                                                   ([50, 10, 5, -1], 57, 0), ([2 ** 31 - 1, 0, 4, 10], 47, 10), ([20, 57, 30, 40], 20, 27)])
+def test_bounds_outside_the_batch_and_out_of_order(paged, dev, starts, untouched, once):
+    """The rows that stay with one sequence are right, those with none are left alone."""
+    case = _case([4, 50, 3], [60, 120, 60], 4, 2, 64, 16)
+    assert _check_bounds(paged, dev, case, torch.tensor(starts, dtype=I)) == [untouched, once]
+
+
+@pytest.mark.parametrize("d", [16, 144])
+@pytest.mark.parametrize("width", [44, 200])
+@pytest.mark.parametrize("seqs", [60, 500, 600])
+def test_many_bounds_out_of_order(paged, dev, d, width, seqs):
+    """Bounds in order but for some neighbours, among few sequences and many, with whole tiles and (where the table is wide)
+    with the partition: every row of one sequence is attended as that sequence's."""
+    g = torch.Generator().manual_seed(seqs + width)
+    q, kc, vc, tables, _, _ = _case([700], [700], 1, 1, d, 16, seed=d)
+    tables = torch.cat([tables[:, :44], torch.zeros(1, width - 44, dtype=I)], 1).clamp(max=kc.shape[0] - 1)
+    starts = torch.randint(0, 701, (seqs + 1,), generator=g).sort().values.int()
+    starts[0], starts[-1] = -5, 720
+    for i in torch.randperm(seqs - 2, generator=g)[:12].tolist():
+        starts[i + 1], starts[i + 2] = starts[i + 2].clone(), starts[i + 1].clone()
+    ctx = 660 + torch.arange(seqs, dtype=I) % 40
+    kc, vc = kc.nan_to_num(0, 0, 0), vc.nan_to_num(0, 0, 0)
+    untouched, once = _check_bounds(paged, dev, (q, kc, vc, tables.expand(seqs, -1).contiguous(), ctx, None), starts)
+    assert untouched == 0 and once >= 300
+
+
+def test_every_row_joined_by_log_sum_exp(paged, dev):
+    """Every row's context in two parts, attended on their own and joined: the keys of the first 320 tokens and the row's own
+    chunk as far as it, against the whole and against the definition.
+
+    A log-sum-exp is within `_tolerances` of its own; the joined one adds two exponentials and a logarithm in fp32 (2^-20).  A weight of the
+    join is off by as much as the log-sum-exps are, and each part by its own tolerance."""
+    n, past_len, block = 12, 320, 32
+    case = q, kc, vc, tables, ctx, starts = _case([n], [n + past_len], 4, 2, 64, block, seed=9)
+    tables = tables.clamp(max=kc.shape[0] - 1)
+    on = lambda *ts: [t.to(dev) for t in ts]  # noqa: E731
+    ref = S.paged_attention_chunk_ref(q, kc, vc, tables, ctx, starts)
+    whole, lse = paged.paged_attention_chunk(*on(q, kc, vc, tables, ctx, starts), return_lse=True)
+    one_each = torch.arange(n + 1, dtype=I)
+    past, past_lse = paged.paged_attention_chunk(*on(q, kc, vc, tables.expand(n, -1).contiguous(), torch.full((n,), past_len, dtype=I), one_each),
+                                                 return_lse=True)
+    own, own_lse = paged.paged_attention_chunk(*on(q, kc, vc, tables[:, past_len // block:].contiguous(), ctx - past_len, starts), return_lse=True)
+    total = torch.logaddexp(past_lse, own_lse)
+    joined = past.float() * (past_lse - total).exp()[..., None] + own.float() * (own_lse - total).exp()[..., None]
+    tol_o, tol_l = _tolerances(case, None, None, 64 ** -0.5, 0, ref)
+    assert ((total.cpu().double() - ref[1]).abs() <= 2 * tol_l + 2.0 ** -20).all()
+    assert ((lse.cpu().double() - ref[1]).abs() <= tol_l).all()
+    largest = float(vc.nan_to_num(0, 0, 0).abs().max())
+    assert ((joined.cpu().double() - ref[0]).abs() <= 2 * tol_o + (3 * tol_l.max() + 2.0 ** -19) * largest).all()
+    assert ((whole.cpu().double() - ref[0]).abs() <= tol_o).all()
