@@ -25,7 +25,9 @@
 // Softmax.  In log2 units, fp32.  The reference value of a row moves only when the maximum has grown by more than
 // 2^kSlack over it, so accumulators are rarely rescaled; weights are exp2(s - ref + kLift), which keeps those up to 2^-20 of
 // the largest normal numbers when they are rounded to fp16 for the product, at most 2^(kLift + kSlack) = 2^14.  Their sum is
-// taken before that rounding.
+// taken before that rounding.  It is the only one to fewer than 32 bits in front of the result's: the matrix core takes both operands in
+// 16 bits, and weights in two halves would double the second product.  It costs 2.6-2.9e-4 of the result against 64 bits instead of
+// 2.1e-4.  A row whose reference value is beyond kChunkFar has its scores rounded before that is taken off (chunk_softmax).
 //
 // Masked places.  Scores out of sight are replaced, not added to, so their K may hold anything.  V rows behind the context
 // are zeroed on the way in; a V row that some rows of the tile see and others must not, and that holds an infinity or NaN,
@@ -33,13 +35,16 @@
 // of the products and added to the results (chunk_add_not_finite).
 //
 // What it measured (MI355X; 32 query and 8 kv heads of 128 elements, pages of 128 tokens unless said otherwise):
-//    4096 tokens over 32768 keys   1720-1800 us over the cards seen, 1.15-1.20 PFLOP/s (a library matrix product of 8192^3 reached
+//    4096 tokens over 32768 keys   1720-1820 us over the cards seen, 1.13-1.20 PFLOP/s (a library matrix product of 8192^3 reached
 //                                  1.47): bound by the matrix core under the power limit (1.9 GHz; busy 0.59 of the cycles; the same
 //                                  loop with the softmax left out takes 1250 us)
 //    16 tokens over 131079 keys    98 us, 5.5 TB/s of K and V (a copy of 1 GiB reached 5.0 read and written): bound by HBM, 90 us,
 //                                  and by joining partial results
 //    24 sequences, 14 of one token and 10 of 253 to 470, window 1024, 16 + 16 heads of 80, pages of 16 tokens
-//                                  86 us: 304 tiles and 224 single rows on 256 CUs, two rounds of about 40 us of 20 steps each
+//                                  87-90 us: 304 tiles and 224 single rows on 256 CUs, two rounds of about 40 us of 20 steps each,
+//                                  because a tile has up to 256 rows whatever the batch
+//    first prompts of 1000, 2000 and 4000 tokens   33, 58 and 140 us, 0.17, 0.38 and 0.64 of the library product's rate: 128, 256
+//                                  and 512 tiles of that height on 256 CUs
 //    4 sequences of 2 to 5 tokens over up to 704 keys   12.7 us: latency, four steps of about 1.2 us on 32 CUs between 3 us that
 //                                  find and load the rows and 3 us that join and store them
 #pragma once
@@ -871,7 +876,7 @@ __device__ __forceinline__ void chunk_run_stream(ChunkArgsRef a, const ChunkTile
   }
   // [wave][row][four d], the groups of four d in an order that depends on the row: rows are as long as the banks are wide, so
   // the same group of 16 rows, which a wave writes together, would fall into the same banks (12.7 us instead of 15.6 for four
-  // sequences of five tokens over up to 1004 keys)
+  // sequences of 2 to 5 tokens over up to 704 keys)
   f32x4* acc = reinterpret_cast<f32x4*>(lds);
   constexpr int kRow = Dims::kJoinBlocks * 4;
   static_assert((kRow & (kRow - 1)) == 0, "groups of a row are told apart by their bits");

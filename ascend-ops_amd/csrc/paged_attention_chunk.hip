@@ -74,9 +74,11 @@ static bool chunk_sizes_ok(int64_t tokens, int64_t seqs, int64_t num_heads, int6
 }
 
 // Where contexts may be longer than kChunkWorth units (by what a row of the block table can hold) the kernel that can cut tiles is
-// taken, which looks at the lengths: it costs a small call 3 us (4 sequences of 2 to 5 tokens over up to 1004 keys: 16.8 and 20.0 us,
+// taken, which looks at the lengths: it costs a small call 4.5 us (4 sequences of 2 to 5 tokens over up to 1004 keys: 14.4 and 19.0 us,
 // of which the launch that finds nothing to join is most), and where contexts are long it saves much more (16 tokens over 131079
-// keys: 1700 and 98 us).  All tiles' units together are counted in 32 bits.
+// keys: 1700 and 98 us).  All tiles' units together are counted in 32 bits, and every workgroup plans all tiles in its LDS, which has room
+// for kChunkMaxTiles: beyond that tiles stay whole, and one long context among many short ones is what the call waits for (one token
+// each of 999 sequences of 100 keys and 4 tokens over 131072 keys 576 us, of 1014 sequences and the same 1230).
 static ChunkPlan chunk_plan(int64_t tokens, int64_t seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                             int64_t block_size, int64_t max_pages) {
   const int64_t group = num_heads / num_kv_heads, cus = device_cu_count(), tile_rows = chunk_rows((int)head_dim);

@@ -432,7 +432,7 @@ __device__ __forceinline__ int given_out(int upto, int free, int* sums) { return
 // Counts in `held` (LDS) the pages that children share with their parents: the first `full` pages of row `row` for the child
 // that each thread stands for (row 0 where full is 0).  A thread takes (child, page) pairs, eight at a time, whose loads are in
 // flight together: a thread per child, which walks its pages one after the other, took 304 us for one child of 4000 pages and
-// 81 for 1000; so they take 9.2 and 8.2, in two launches, with a workgroup per child, 12.4 and 8.5.
+// 81 for 1000; so they take 8.5 and 7.4, in two launches, with a workgroup per child, 12.4 and 9.1.
 __device__ __forceinline__ void hold_shared_pages(const Tables& t, int row, int full, int children, int32_t num_blocks, int* rows,
                                                   int* fulls, int* held, int* sums) {
   constexpr int kDeep = 8, kThreads = kRowWaves * kWave;
@@ -653,11 +653,11 @@ static PlanOut plan_layout(void* workspace, int64_t num_blocks) {
 }
 
 // Sides of the rule (us, one launch and two): a beam step of 4 sequences in a pool of 96 pages, three calls, 17 and 23; 128 children of
-// short sequences in a pool of 4096 pages 9 and 11, 256 in one of 1200 pages 10 and 12, of 4096 pages 14 and 11, 512 17-22 and 14,
-// 2000 91 and 33: every workgroup looks at all requests and all counts.  Extending 256 sequences 8 and 10.
-// `most` entries of the requests' rows: the pages of forks and of sequences that end are counted by one workgroup, 4000 of them in 9.2
-// and 9.2-12.0 (fork), 5.0 and 6.5-10.1 (free), 16000 in 15.7 and 9.3, 11.6 and 6.6; rows are extended by a workgroup each, 16000
-// entries in 7.9-9.9 and 8.2-8.5.
+// short sequences in a pool of 4096 pages 7.5 and 9.0, 256 7.9 and 9.1, 512 17-22 and 14, 2000 91 and 33: every
+// workgroup looks at all requests and all counts.  Extending 256 sequences 6.0 and 8.3.
+// `most` entries of the requests' rows: the pages of forks and of sequences that end are counted by one workgroup, 4000 of them in 8.5
+// and 9.0-12.4 (fork), 5.0 and 6.5-10.0 (free), 16000 in 15.7 and 9.3, 11.6 and 6.6; rows are extended by a workgroup each, 16000
+// entries in 6.0-7.9 and 8.2-8.6.
 static bool small_pool(int64_t num_blocks, int64_t requests, int64_t max_pages, int64_t most) {
   return num_blocks <= kSmallPool && requests <= kSmallRequests && requests * max_pages <= most;
 }
