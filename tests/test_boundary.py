@@ -215,3 +215,16 @@ def test_product_package_does_not_import_the_oracle():
             if f.endswith((".py", ".hip", ".h", ".cpp")):
                 text = open(os.path.join(dirpath, f)).read()
                 assert "oracle" not in text, f"{f} mentions the oracle"
+
+
+def test_recorded_traffic_belongs_to_the_present_kernel_source():
+    """bench.py reports the recorded HBM traffic of the decode attention only for the source it was measured on: after a
+    change of that source it is measured again, by the commands in the record."""
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("aops_bench", os.path.join(ROOT, "bench.py"))
+    bench = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(bench)
+    record = open(os.path.join(ROOT, "profiles", "pa_decode_config5_hbm_traffic.txt")).read()
+    assert re.search(r"^kernel_source_digest: (\w+)$", record, re.M).group(1) == bench.kernel_source_digest()
+    assert int(re.search(r"^\s*traffic_bytes_per_launch: (\d+)$", record, re.M).group(1)) > 0
