@@ -38,8 +38,8 @@ def paged_attention_chunk(
     ``q [tokens, heads, D]`` holds the new tokens of all sequences one after the other; sequence ``b`` has the rows
     ``query_starts[b]:query_starts[b+1]`` (int32 ``[sequences + 1]``), which are the last tokens of its ``context_lens[b]``.  A
     row sees the keys up to its own position, only the last ``window`` of them where ``window > 0``; kv head and page of a key
-    as in ``ops.paged_attention``, ``scale`` (positive, at most 2^56) 1/sqrt(D) if not given.  A row that sees nothing (a context shorter than the new
-    tokens) is 0.  Lengths and tables are read on the device only.
+    as in ``ops.paged_attention``, ``scale`` (positive, at most 2^56) 1/sqrt(D) if not given.  A row that sees nothing (a
+    context shorter than the new tokens) is 0.  Lengths and tables are read on the device only.
 
     Returns ``o`` like ``q``, with ``return_lse`` also the natural log-sum-exp of the scaled scores, fp32 ``[tokens, heads]``
     (-inf where nothing is seen), by which results over parts of a context can be joined.  Rows of no sequence (a batch padded

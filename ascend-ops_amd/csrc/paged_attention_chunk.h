@@ -963,7 +963,8 @@ __device__ __forceinline__ bool chunk_find(ChunkArgsRef a, int tile, int* shared
   for (uint32_t base = 0; base < (uint32_t)a.seqs; base += PER * kWave * WAVES) {
     const uint32_t own = base + (alone ? lane : threadIdx.x) * PER, first = min(own, (uint32_t)(a.seqs - PER));
     // A lane's bounds lie next to each other and are on their way at once (a pair for each sequence, under a condition of its own, was
-    // waited for: 512 decoding sequences 169 us instead of 164, 8000 2.74 ms instead of 2.66).  The last lanes with sequences read the last PER and leave out those in front of their own.
+    // waited for: 512 decoding sequences 169 us instead of 164, 8000 2.74 ms instead of 2.66).  The last lanes with sequences read the
+    // last PER and leave out those in front of their own.
     int bounds[PER + 1], tiles[PER], mine = 0;
 #pragma unroll
     for (int i = 0; i <= PER; ++i) bounds[i] = a.query_starts[first + i];

@@ -530,3 +530,25 @@ def test_every_row_joined_by_log_sum_exp(paged, dev):
     largest = float(vc.nan_to_num(0, 0, 0).abs().max())
     assert ((joined.cpu().double() - ref[0]).abs() <= 2 * tol_o + (3 * tol_l.max() + 2.0 ** -19) * largest).all()
     assert ((whole.cpu().double() - ref[0]).abs() <= tol_o).all()
+
+
+@pytest.mark.parametrize("d", [80, 128, 208])
+@pytest.mark.parametrize("new,ctx", [([9, 1], [700, 300]), ([50], [400]), ([130], [2900])])
+@pytest.mark.parametrize("window", [0, 200])
+def test_rows_near_and_far_in_one_tile(paged, dev, d, new, ctx, window):
+    """Rows whose scores are far from zero next to ordinary ones: those come out as exactly as without them, these inside what
+    their values span."""
+    case = list(_case(new, ctx, 4, 2, d, 16, seed=d))
+    far = torch.arange(sum(new)) % 5 == 3
+    case[0] = torch.where(far[:, None, None], (case[0].double() * 20000).clamp(-60000, 60000).half(), case[0])
+    ref = S.paged_attention_chunk_ref(*case, window=window)
+    o, lse = paged.paged_attention_chunk(*(t.to(dev) for t in case), window=window, return_lse=True)
+    o, lse = o.cpu().double(), lse.cpu().double()
+    assert bool(o.isfinite().all() and lse.isfinite().all())
+    assert o.abs().max() <= case[2][case[2].isfinite()].abs().max()
+    # a far row's log-sum-exp is its largest score, to the rounding of D products and their sum
+    assert ((lse[far] - ref[1][far]).abs() <= ref[1][far].abs().clamp(min=1) * (d + 4) * 2.0 ** -20).all()
+    near = [case[0][~far], *case[1:]]
+    tol_o, tol_l = _tolerances(near, None, None, d ** -0.5, window, (ref[0][~far], ref[1][~far]))
+    assert ((o[~far] - ref[0][~far]).abs() <= tol_o).all()
+    assert ((lse[~far] - ref[1][~far]).abs() <= tol_l).all()
